@@ -228,7 +228,7 @@ def prepare(case, seed):
         vkb = _vkb()
         st["cache"] = vkb.KvCache(st["k"], st["v"], st["ks"], st["vs"])
         if op == "attention":
-            st["work"] = vkb.attention_workspace(st["cache"], hq)
+            st["work"] = vkb.attention_workspace(st["cache"])
     return st
 
 
