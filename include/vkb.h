@@ -133,6 +133,79 @@ int vkb_gemm_q8_tc_f32(const void* q, const void* s, const void* x, float* y, in
 int vkb_gemm_tc(int fmt, const void* q, const void* s, const void* x, void* y, int out_f32, int N, int K, int M,
                 vkb_stream_t stream);
 
+/* ---- between the products of a decode step: norm, rotary append to an 8-bit cache, attention over it, sampling ----------
+ * No counterpart in the reference, which holds the quantised products alone; these take their outputs (fp16 or fp32)
+ * and feed their inputs (fp16). Element types are VKB_DT_*; rows may be strided where a leading dimension (ld*, in
+ * elements) is given. Every call is one launch, allocates nothing and may be captured in a graph: lengths, offsets and
+ * the page table are read on the device, so a captured step stays right while sequences grow. */
+enum { VKB_DT_F16 = 0, VKB_DT_BF16 = 1, VKB_DT_F32 = 2 };
+
+/* r = x + res (res may be null: r = x), y = r / sqrt(mean(r^2) + eps) * w, computed in fp32 from the unrounded r and
+ * rounded once. x (type dt, rows ldx apart), w [d] and y [T][d] have type dt; res and res_out [T][d] have type res_dt;
+ * res_out (may be null, may be res) receives r. q (int8 [T][d]) and s (fp16 [T][d/32]), both or neither: y in the
+ * Q8 format above, quantised by vkb_quantize's rule from the unrounded y (d % 32 == 0; vkb_dequant reads it). y may be
+ * null when q is given. y may be x when ldx == d. */
+int vkb_rms_norm(int dt, const void* x, long long ldx, const void* res, void* res_out, int res_dt, const void* w,
+                 float eps, void* y, void* q, void* s, int T, int d, vkb_stream_t stream);
+
+/* A paged key/value cache in 8 bits, in caller-owned device memory: codes uint8 [pages][heads][page][dim], stored as
+ * code + 128 (-127..127; 16-byte aligned), one fp32 scale >= 0 per page and head, [pages][heads]; value = code * scale.
+ * page: 16, 32, 64 or 128 tokens; dim: a multiple of 16 up to 256. A sequence's token p is in slot p % page of page
+ * table[b][p / page] (int32 [B][table_ld]); pages may come in any order and may be shared, except that a page being
+ * appended to belongs to one sequence.
+ * The calls below take lens [B]: each sequence's length including the call's new tokens, and cu [B + 1]: sequence b's
+ * rows are cu[b] .. cu[b + 1] - 1 of the call's T rows, its last cu[b + 1] - cu[b] tokens (cu null: one row per
+ * sequence, T == B). A sequence of length 0 is an idle one: nothing is written for it and its attention output is
+ * zero. Lengths, offsets and pages outside their arrays are skipped and raise bit 16 of vkb_device_status. */
+typedef struct vkb_kv_cache {
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+    int pages, heads, page, dim;
+} vkb_kv_cache_t;
+
+/* Rotates q and k, and writes k and v into the cache: q_out [T][q_heads * dim] = R(pos) q, token rows of k and v go to
+ * their slots as codes. rot elements of each head are rotated (even; 0: none): VKB_ROPE_HALF pairs element i with
+ * i + rot / 2, VKB_ROPE_INTERLEAVED 2i with 2i + 1. turns [rot / 2] (device): turns per position of each pair as a
+ * 64-bit fraction of a turn, round(frequency / 2 pi * 2^64) (long-context scalings are other frequencies); mscale
+ * multiplies cos and sin. Positions: pos [T], or the token's place in its sequence where pos is null. Types of q, k, v
+ * and q_out: dt; heads of a row are adjacent, rows ldq, ldk, ldv, ldqo apart (views of one fused row). q_out may be q
+ * (same rows). q_heads 0: no q.
+ * A page's scale becomes max(scale of the tokens it held before, largest new magnitude / 127), new codes are
+ * rint(x / scale) (infinities: +-127, not part of the scale; NaN: 0), and codes held before follow a growing scale as
+ * rint(code * old / new). The first token written to a page (slot 0) starts its scale anew. */
+enum { VKB_ROPE_HALF = 0, VKB_ROPE_INTERLEAVED = 1 };
+int vkb_rope_append(const vkb_kv_cache_t* cache, const int32_t* table, int table_ld, const int32_t* lens,
+                    const int32_t* cu, int B, int T, int dt, const void* q, long long ldq, void* q_out, long long ldqo,
+                    int q_heads, const void* k, long long ldk, const void* v, long long ldv, const int32_t* pos,
+                    const uint64_t* turns, int rot, int layout, float mscale, vkb_stream_t stream);
+/* Cached tokens as values: row i of k and v [n][heads][dim] (type dt, 16-byte aligned) is token pos[i] of sequence
+ * seq[i] (zeros and the status bit for one that is not in the table). */
+int vkb_kv_read(const vkb_kv_cache_t* cache, const int32_t* table, int table_ld, int B, const int32_t* seq,
+                const int32_t* pos, int n, int dt, void* k, void* v, vkb_stream_t stream);
+
+/* out[t][h] = sum_j softmax_j(scale * q[t][h] . k_j) v_j over the cache, query head h on kv head h / (q_heads / heads).
+ * Query row i of a sequence's n rows is at position len - n + i and sees the keys at positions up to its own, with
+ * window > 0 only the last `window` of them; a row that sees no key is zero. q and out: fp16 or bf16, 16-byte aligned
+ * rows. work: vkb_attention_work_bytes(dim) bytes (for the current device), 16-byte aligned, zeroed by the caller once
+ * before its first use; calls leave it ready for the next one. Calls that overlap in time need a workspace each. */
+size_t vkb_attention_work_bytes(int dim);
+int vkb_attention(const vkb_kv_cache_t* cache, const int32_t* table, int table_ld, const int32_t* lens,
+                  const int32_t* cu, int B, int T, int dt, const void* q, long long ldq, void* out, long long ldo,
+                  int q_heads, float scale, int window, void* work, size_t work_bytes, vkb_stream_t stream);
+
+/* One token per row of logits [B] x [V] (type dt, rows ld apart), from given uniform numbers u [B] in [0, 1). Tokens are
+ * ordered by (logit descending, index ascending); top_k [B] keeps the first k (<= 0: all), top_p [B] the shortest
+ * prefix of those whose weight exp((logit - max) / temperature) reaches p of theirs (>= 1: all; <= 0: the first),
+ * min_p [B] those whose weight is at least min_p of the largest; the token is the first in index order at which the
+ * running weight of the kept ones exceeds u times their sum. temperature [B] <= 0: the first token of the order. Null
+ * arrays: temperature 1, no top-k, top-p or min-p. NaN logits are never taken; a row with nothing to take gives token -1
+ * and probability 0. token int32 [B]; prob fp32 [B] (may be null): the token's share of the kept weight. V up to 393216. */
+int vkb_sample(int dt, const void* logits, long long ld, int B, int V, const float* temperature, const int32_t* top_k,
+               const float* top_p, const float* min_p, const float* u, int32_t* token, float* prob,
+               vkb_stream_t stream);
+
 /* ---- multi-GPU: one process (and one rank) per GPU ---------------------------------------------------------------------
  * No counterpart in the reference, which runs on one GPU: these shard the MoE (by experts) and the prompt GEMM (by
  * weight rows) over the GPUs of one node. A communicator wraps one NCCL rank on the device that is current at vkb_comm_init. Collective entry points must be
@@ -227,7 +300,7 @@ int vkb_graph_destroy(void* graph_exec);
 const char* vkb_strerror(int code);
 /* Synchronises the current device, returns (and clears) the device-side status bits that kernels raise when a bounded
  * wait gives up (1 = pipeline wait timeout, 2 = drain timeout, 4 = peer timeout) or a peer rank reports its part of a
- * fused multi-GPU call missing (8). 0 = healthy. */
+ * fused multi-GPU call missing (8), or finds a length, offset or page index outside its array (16). 0 = healthy. */
 int vkb_device_status(unsigned int* bits);
 /* Enable (1) or disable (0) programmatic dependent launch for later calls on this host thread; returns the old value. */
 int vkb_set_pdl(int enable);

@@ -1,0 +1,94 @@
+// vkb_attention: argument checks, choice of the kernel, launch. The kernels: attn_token.cuh (few query rows per kv head).
+#include <mutex>
+
+#include "attn_token.cuh"
+
+namespace vkb {
+
+VKB_STATUS_ACCESSOR(status_take_attn)
+
+int kv_cache_check(const vkb_kv_cache_t* c, const int32_t* table, int table_ld);   // kv_cache.cu
+
+// Head dimension as the kernels hold it.
+static int attn_dt(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+// The largest partial result of a block: rows x (dimension, maximum and sum), of any variant.
+static size_t attn_part_floats(int dt) {
+    return (size_t)(4096 / dt) * (dt + 2);
+}
+
+template <int DT, int MT, typename T>
+static int launch_token(const vkb_kv_cache_t* c, const AttnArgs& a, int dev, cudaStream_t st) {
+    using C = TkCfg<DT, MT>;
+    auto kern = attn_token_kernel<DT, MT, T>;
+    static std::once_flag once[kMaxDevices];
+    static cudaError_t err[kMaxDevices];
+    std::call_once(once[dev], [&] {
+        err[dev] = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::BYTES);
+    });
+    if (err[dev] != cudaSuccess) return -(int)err[dev];
+    CUtensorMap tk, tv;
+    const uint64_t rows = (uint64_t)c->pages * c->heads * c->page;
+    const uint32_t pb = c->page < AT_KT ? c->page : AT_KT;
+    const CUtensorMapSwizzle swz = DT == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
+    if (int r = get_tmap_2d(&tk, c->k, rows, c->dim, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, C::HB, pb, swz)) return r;
+    if (int r = get_tmap_2d(&tv, c->v, rows, c->dim, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, C::HB, pb, swz)) return r;
+    return launch_pdl(kern, dim3((unsigned)device_info(dev).sm_count), dim3(TK_THREADS), C::BYTES, st, 1, tk, tv, a);
+}
+
+template <typename T>
+static int attn_dispatch(const vkb_kv_cache_t* c, const AttnArgs& a, int dev, cudaStream_t st) {
+    // Query rows per sequence and kv head, on average: the row tile that holds them (a tile of 16 rows per product).
+    const long long rows = ((long long)a.T + a.B - 1) / a.B * a.G;
+    switch (attn_dt(c->dim)) {
+        case 64:
+            return rows <= 16 ? launch_token<64, 1, T>(c, a, dev, st)
+                   : rows <= 32 ? launch_token<64, 2, T>(c, a, dev, st) : launch_token<64, 4, T>(c, a, dev, st);
+        case 128:
+            return rows <= 16 ? launch_token<128, 1, T>(c, a, dev, st) : launch_token<128, 2, T>(c, a, dev, st);
+        default: return launch_token<256, 1, T>(c, a, dev, st);
+    }
+}
+
+constexpr size_t ATTN_CNT_BYTES = 4096;   // arrival counters: one per block of the grid (one per SM)
+
+}  // namespace vkb
+
+using namespace vkb;
+
+extern "C" size_t vkb_attention_work_bytes(int dim) {
+    int dev = 0;
+    if (dim < 16 || dim > 256 || dim % 16 || current_device(&dev)) return 0;
+    return ATTN_CNT_BYTES + (size_t)device_info(dev).sm_count * 2 * attn_part_floats(attn_dt(dim)) * sizeof(float);
+}
+
+extern "C" int vkb_attention(const vkb_kv_cache_t* c, const int32_t* table, int table_ld, const int32_t* lens,
+                             const int32_t* cu, int B, int T, int dt, const void* q, long long ldq, void* out,
+                             long long ldo, int q_heads, float scale, int window, void* work, size_t work_bytes,
+                             vkb_stream_t stream) {
+    if (int r = kv_cache_check(c, table, table_ld)) return r;
+    if (!lens || B < 1 || T < 0 || (!cu && T != B) || window < 0) return VKB_EINVAL;
+    if (dt != VKB_DT_F16 && dt != VKB_DT_BF16) return dt == VKB_DT_F32 ? VKB_EUNSUPPORTED : VKB_EINVAL;
+    if (q_heads < 1 || q_heads % c->heads) return VKB_EINVAL;
+    if (T == 0) return 0;
+    const long long row = (long long)q_heads * c->dim;
+    if (!q || !out || ldq < row || ldo < row) return VKB_EINVAL;
+    if (!work || !aligned_to(work, 16) || work_bytes < vkb_attention_work_bytes(c->dim)) return VKB_EINVAL;
+    if (!aligned_to(q, 16) || !aligned_to(out, 16) || ldq % 8 || ldo % 8) return VKB_EUNSUPPORTED;
+    if ((long long)T * (q_heads / c->heads) > 0x7fffffffll) return VKB_EUNSUPPORTED;
+    int dev = 0;
+    if (int r = current_device(&dev)) return r;
+    if ((size_t)device_info(dev).sm_count * sizeof(unsigned) > ATTN_CNT_BYTES) return VKB_EUNSUPPORTED;
+    AttnArgs a{};
+    a.table = table; a.lens = lens; a.cu = cu;
+    a.ks = c->k_scale; a.vs = c->v_scale;
+    a.q = q; a.out = out;
+    a.cnt = (unsigned*)work;
+    a.part = (float*)((uint8_t*)work + ATTN_CNT_BYTES);
+    a.ldq = ldq; a.ldo = ldo;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    a.B = B; a.T = T; a.heads = c->heads; a.G = q_heads / c->heads; a.dim = c->dim; a.pages = c->pages;
+    a.page_log2 = c->page == 16 ? 4 : c->page == 32 ? 5 : c->page == 64 ? 6 : 7;
+    a.table_ld = table_ld; a.window = window;
+    cudaStream_t st = (cudaStream_t)stream;
+    return dt == VKB_DT_F16 ? attn_dispatch<__half>(c, a, dev, st) : attn_dispatch<__nv_bfloat16>(c, a, dev, st);
+}

@@ -20,7 +20,7 @@ namespace vkb {
 VKB_STATUS_ACCESSOR(status_take_qmv)
 
 StatusList status_accessors() {
-    static const StatusTake list[] = {status_take_qmv, status_take_comm};
+    static const StatusTake list[] = {status_take_qmv, status_take_comm, status_take_kv, status_take_attn};
     return {list, list + sizeof(list) / sizeof(list[0])};
 }
 

@@ -51,6 +51,8 @@ bool pdl_stream_ok(cudaStream_t st);
 using StatusTake = int (*)(unsigned*);
 int status_take_qmv(unsigned* bits);
 int status_take_comm(unsigned* bits);
+int status_take_kv(unsigned* bits);
+int status_take_attn(unsigned* bits);
 struct StatusList {
     const StatusTake* b;
     const StatusTake* e;

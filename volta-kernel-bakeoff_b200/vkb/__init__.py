@@ -84,7 +84,7 @@ def lib() -> ctypes.CDLL:
 
 def _register_optional(L) -> None:
     """Entry points added by later parts of the library (bound when present)."""
-    vp, i = ctypes.c_void_p, ctypes.c_int
+    vp, i, ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
     opt = {
         "vkb_gemm_q4_tc": ([vp, vp, vp, vp, i, i, i, vp], i),
         "vkb_gemm_q4_tc_f32": ([vp, vp, vp, vp, i, i, i, vp], i),
@@ -120,6 +120,13 @@ def _register_optional(L) -> None:
         "vkb_graph_launch": ([vp, vp], i),
         "vkb_graph_destroy": ([vp], i),
         "vkb_plan_describe": ([i, i, i, i, i, i, i, i, vp], i),
+        "vkb_rms_norm": ([i, vp, ll, vp, vp, i, vp, ctypes.c_float, vp, vp, vp, i, i, vp], i),
+        "vkb_rope_append": ([vp, vp, i, vp, vp, i, i, i, vp, ll, vp, ll, i, vp, ll, vp, ll, vp, vp, i, i, ctypes.c_float,
+                             vp], i),
+        "vkb_kv_read": ([vp, vp, i, i, vp, vp, i, i, vp, vp, vp], i),
+        "vkb_attention_work_bytes": ([i], ctypes.c_size_t),
+        "vkb_attention": ([vp, vp, i, vp, vp, i, i, i, vp, ll, vp, ll, i, ctypes.c_float, i, vp, ctypes.c_size_t, vp], i),
+        "vkb_sample": ([i, vp, ll, i, i, vp, vp, vp, vp, vp, vp, vp, vp], i),
     }
     for name, (args, res) in opt.items():
         if hasattr(L, name):
@@ -409,3 +416,17 @@ def to_device_packed(packed: np.ndarray, device="cuda"):
 def to_device_f16(bits: np.ndarray, device="cuda"):
     torch = _torch()
     return torch.from_numpy(np.ascontiguousarray(bits).view(np.int16).copy()).to(device).view(torch.float16)
+
+
+# ---- the operators between the products (step.py; it needs torch, so it is imported when first used) ---------------
+
+_STEP = ("rms_norm", "rope_turns", "rope_append", "KvCache", "kv_read", "attention", "attention_workspace", "sample")
+
+
+def __getattr__(name: str):
+    if name not in _STEP:
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    from . import step
+    for n in _STEP:
+        globals()[n] = getattr(step, n)
+    return globals()[name]
