@@ -1,6 +1,8 @@
-// vkb_attention: argument checks, choice of the kernel, launch. The kernels: attn_token.cuh (few query rows per kv head).
+// vkb_attention: argument checks, choice of the kernel, launch. The kernels: attn_token.cuh (few query rows per kv head),
+// attn_prompt.cuh (many).
 #include <mutex>
 
+#include "attn_prompt.cuh"
 #include "attn_token.cuh"
 
 namespace vkb {
@@ -13,7 +15,7 @@ int kv_cache_check(const vkb_kv_cache_t* c, const int32_t* table, int table_ld);
 static int attn_dt(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 // The largest partial result of a block: rows x (dimension, maximum and sum), of any variant.
 static size_t attn_part_floats(int dt) {
-    return (size_t)(4096 / dt) * (dt + 2);
+    return (size_t)(dt == 256 ? 128 : 256) * (dt + 2);   // the prompt kernel's tile is the larger one
 }
 
 template <int DT, int MT, typename T>
@@ -24,6 +26,10 @@ static int launch_token(const vkb_kv_cache_t* c, const AttnArgs& a, int dev, cud
     static cudaError_t err[kMaxDevices];
     std::call_once(once[dev], [&] {
         err[dev] = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::BYTES);
+        // the kernel's register split needs the registers that the block is launched with
+        cudaFuncAttributes fa;
+        if (err[dev] == cudaSuccess) err[dev] = cudaFuncGetAttributes(&fa, kern);
+        if (err[dev] == cudaSuccess && fa.numRegs * TK_THREADS < 128 * 40 + 256 * 232) err[dev] = cudaErrorInvalidConfiguration;
     });
     if (err[dev] != cudaSuccess) return -(int)err[dev];
     CUtensorMap tk, tv;
@@ -35,10 +41,31 @@ static int launch_token(const vkb_kv_cache_t* c, const AttnArgs& a, int dev, cud
     return launch_pdl(kern, dim3((unsigned)device_info(dev).sm_count), dim3(TK_THREADS), C::BYTES, st, 1, tk, tv, a);
 }
 
+template <int DT, typename T>
+static int launch_prompt(const vkb_kv_cache_t* c, const AttnArgs& a, int dev, cudaStream_t st) {
+    using C = PrCfg<DT>;
+    auto kern = attn_prompt_kernel<DT, T>;
+    static std::once_flag once[kMaxDevices];
+    static cudaError_t err[kMaxDevices];
+    std::call_once(once[dev], [&] {
+        err[dev] = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::BYTES);
+    });
+    if (err[dev] != cudaSuccess) return -(int)err[dev];
+    return launch_pdl(kern, dim3((unsigned)device_info(dev).sm_count), dim3(PR_THREADS), C::BYTES, st, 1, a,
+                      (const uint8_t*)c->k, (const uint8_t*)c->v);
+}
+
 template <typename T>
 static int attn_dispatch(const vkb_kv_cache_t* c, const AttnArgs& a, int dev, cudaStream_t st) {
     // Query rows per sequence and kv head, on average: the row tile that holds them (a tile of 16 rows per product).
     const long long rows = ((long long)a.T + a.B - 1) / a.B * a.G;
+    if (rows > 64) {
+        switch (attn_dt(c->dim)) {
+            case 64: return launch_prompt<64, T>(c, a, dev, st);
+            case 128: return launch_prompt<128, T>(c, a, dev, st);
+            default: return launch_prompt<256, T>(c, a, dev, st);
+        }
+    }
     switch (attn_dt(c->dim)) {
         case 64:
             return rows <= 16 ? launch_token<64, 1, T>(c, a, dev, st)
@@ -66,7 +93,7 @@ extern "C" int vkb_attention(const vkb_kv_cache_t* c, const int32_t* table, int 
                              long long ldo, int q_heads, float scale, int window, void* work, size_t work_bytes,
                              vkb_stream_t stream) {
     if (int r = kv_cache_check(c, table, table_ld)) return r;
-    if (!lens || B < 1 || T < 0 || (!cu && T != B) || window < 0) return VKB_EINVAL;
+    if (!lens || B < 1 || T < 0 || (!cu && T != B) || window < 0 || !(scale >= 0.f)) return VKB_EINVAL;
     if (dt != VKB_DT_F16 && dt != VKB_DT_BF16) return dt == VKB_DT_F32 ? VKB_EUNSUPPORTED : VKB_EINVAL;
     if (q_heads < 1 || q_heads % c->heads) return VKB_EINVAL;
     if (T == 0) return 0;

@@ -3,7 +3,7 @@
 //
 // A work item is one sequence, one kv head and one tile of ROWS query rows; row r of a sequence is query token r / G,
 // head h G + r % G (G = q heads per kv head), so that the heads sharing a kv head read its codes once. An item's units
-// are its tiles of 64 keys, from the first key that any of its rows sees to the last (an item that sees none has one
+// are its tiles of KT keys, from the first key that any of its rows sees to the last (an item that sees none has one
 // empty unit, which writes its zeros). The units of all items, in order, are dealt out to the thread blocks in equal
 // contiguous runs, worked out on the device from the lengths there: ragged batches balance, nothing is read back to
 // the host, and a captured graph stays right as sequences grow. An item cut by a run's border is a "part" in each
@@ -16,8 +16,6 @@
 #include "step.cuh"
 
 namespace vkb {
-
-constexpr int AT_KT = 64;   // keys per unit
 
 struct AttnArgs {
     const int32_t* table;
@@ -51,23 +49,23 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnArgs& a, int b) {
     return s;
 }
 // The key tiles [t0, t1) of rows [r0, r1) of a sequence (t1 <= t0: no row sees a key).
-__device__ __forceinline__ void attn_tiles(const AttnArgs& a, const AttnSeq& s, int r0, int r1, int* t0, int* t1) {
+template <int KT> __device__ __forceinline__ void attn_tiles(const AttnArgs& a, const AttnSeq& s, int r0, int r1, int* t0, int* t1) {
     const int first = s.len - s.n + r0 / a.G, last = s.len - s.n + (r1 - 1) / a.G;   // token positions
     const int lo = a.window > 0 ? max(0, first - a.window + 1) : 0;
-    *t0 = lo / AT_KT;
-    *t1 = last >= 0 ? (last + AT_KT) / AT_KT : 0;
+    *t0 = lo / KT;
+    *t1 = last >= 0 ? (last + KT) / KT : 0;
     if (*t1 < *t0) *t1 = *t0;
 }
-__device__ __forceinline__ int attn_units(const AttnArgs& a, const AttnSeq& s, int r0, int r1) {
+template <int KT> __device__ __forceinline__ int attn_units(const AttnArgs& a, const AttnSeq& s, int r0, int r1) {
     int t0, t1;
-    attn_tiles(a, s, r0, r1, &t0, &t1);
+    attn_tiles<KT>(a, s, r0, r1, &t0, &t1);
     return max(1, t1 - t0);
 }
 // Units of one head of a sequence.
-template <int ROWS> __device__ __forceinline__ long long attn_head_units(const AttnArgs& a, const AttnSeq& s) {
+template <int ROWS, int KT> __device__ __forceinline__ long long attn_head_units(const AttnArgs& a, const AttnSeq& s) {
     const int rows = s.n * a.G;
     long long u = 0;
-    for (int r = 0; r < rows; r += ROWS) u += attn_units(a, s, r, min(rows, r + ROWS));
+    for (int r = 0; r < rows; r += ROWS) u += attn_units<KT>(a, s, r, min(rows, r + ROWS));
     return u;
 }
 
@@ -94,14 +92,14 @@ __device__ __forceinline__ int attn_owner(long long total, int nb, long long x) 
 }
 
 // All threads of the block: this block's run. sh: 2 + NT / 32 words of 8 bytes of shared memory.
-template <int ROWS, int NT> __device__ __forceinline__ AttnRun attn_run(const AttnArgs& a, long long* sh) {
+template <int ROWS, int KT, int NT> __device__ __forceinline__ AttnRun attn_run(const AttnArgs& a, long long* sh) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int NW = NT / 32;
     AttnRun r;
     long long total = 0, mine0 = 0;
     for (int b = tid; b < a.B; b += NT) {
         const AttnSeq s = attn_seq(a, b);
-        const long long u = a.heads * attn_head_units<ROWS>(a, s);
+        const long long u = a.heads * attn_head_units<ROWS, KT>(a, s);
         if (b == tid) mine0 = u;
         total += u;
     }
@@ -125,7 +123,7 @@ template <int ROWS, int NT> __device__ __forceinline__ AttnRun attn_run(const At
     for (int base = 0; base < a.B; base += NT) {
         const int b = base + tid;
         long long u = mine0;
-        if (base > 0) u = b < a.B ? a.heads * attn_head_units<ROWS>(a, attn_seq(a, b)) : 0;
+        if (base > 0) u = b < a.B ? a.heads * attn_head_units<ROWS, KT>(a, attn_seq(a, b)) : 0;
         long long inc = u;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -151,13 +149,13 @@ template <int ROWS, int NT> __device__ __forceinline__ AttnRun attn_run(const At
     }
     r.b = (int)sh[NW];
     const AttnSeq s = attn_seq(a, r.b);
-    const long long per = attn_head_units<ROWS>(a, s);
+    const long long per = attn_head_units<ROWS, KT>(a, s);
     long long at = sh[NW + 1];
     r.h = (int)(at / per);
     at -= r.h * per;
     const int rows = s.n * a.G;
     for (;; r.r0 += ROWS) {
-        const int u = attn_units(a, s, r.r0, min(rows, r.r0 + ROWS));
+        const int u = attn_units<KT>(a, s, r.r0, min(rows, r.r0 + ROWS));
         if (at < u) break;
         at -= u;
     }
@@ -166,7 +164,7 @@ template <int ROWS, int NT> __device__ __forceinline__ AttnRun attn_run(const At
 }
 
 // The run's next segment; false at its end.
-template <int ROWS> __device__ __forceinline__ bool attn_next(const AttnArgs& a, AttnRun& r, AttnSeg* g) {
+template <int ROWS, int KT> __device__ __forceinline__ bool attn_next(const AttnArgs& a, AttnRun& r, AttnSeg* g) {
     if (r.u >= r.u1) return false;
     AttnSeq s = attn_seq(a, r.b);
     while (s.n == 0) {   // sequences without query tokens have no unit
@@ -182,7 +180,7 @@ template <int ROWS> __device__ __forceinline__ bool attn_next(const AttnArgs& a,
     g->q0 = s.q0;
     g->len = s.len;
     int t0, t1;
-    attn_tiles(a, s, r.r0, r.r0 + g->rows, &t0, &t1);
+    attn_tiles<KT>(a, s, r.r0, r.r0 + g->rows, &t0, &t1);
     const int units = max(1, t1 - t0);
     const int take = (int)min((long long)(units - r.off), r.u1 - r.u);
     g->iu0 = r.u - r.off;

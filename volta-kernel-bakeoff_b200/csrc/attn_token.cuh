@@ -21,6 +21,7 @@
 
 namespace vkb {
 
+constexpr int AT_KT = 64;                            // keys per unit
 constexpr int TK_WARPS = 8;                          // computing warps (two groups of four)
 constexpr int TK_THREADS = 32 * (TK_WARPS + 4);      // and a warpgroup whose first warp streams
 constexpr float TK_P_BIAS = 8.f;                     // p is kept times 2^8
@@ -100,7 +101,7 @@ attn_token_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         prefetch_tmap(&tv);
     }
     pdl_wait();
-    AttnRun run = attn_run<C::ROWS, TK_THREADS>(a, run_sh);   // its barriers also publish the mbarriers
+    AttnRun run = attn_run<C::ROWS, AT_KT, TK_THREADS>(a, run_sh);   // its barriers also publish the mbarriers
     AttnSeg g;
 
     // Registers: 384 threads are launched with 168 each (64512); the streaming warpgroup keeps 40, so that the computing
@@ -112,7 +113,7 @@ attn_token_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         const int pb = min(AT_KT, 1 << a.page_log2);   // keys per box
         int it = 0;
         bool ok = true;
-        while (ok && attn_next<C::ROWS>(a, run, &g)) {
+        while (ok && attn_next<C::ROWS, AT_KT>(a, run, &g)) {
             const int32_t* row = a.table + (long long)g.b * a.table_ld;
             int have = -1, ids = -1;   // this lane's page id of pages [have, have + 32)
             for (int t = g.t0; t < g.t1; ++t, ++it) {
@@ -170,7 +171,7 @@ attn_token_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     float* rowf = reinterpret_cast<float*>(sm + C::row_off);
     int it = 0;
     bool ok = true;
-    while (attn_next<C::ROWS>(a, run, &g)) {
+    while (attn_next<C::ROWS, AT_KT>(a, run, &g)) {
         // ---- q of the tile, in A-fragment order: {a0, a1, a2, a3} of k step ks, row tile mt at [mt][ks][lane]. The k
         // order of a step of 16 is that of the codes' registers: slots 2c, 2c + 1, 2c + 8, 2c + 9 hold 4c .. 4c + 3.
         {
