@@ -13,7 +13,7 @@ import math
 
 import torch
 
-from . import EINVAL, VkbError, _optr, _ptr, _stream, check, lib
+from . import EINVAL, VkbError, check, lib
 
 DT_F16, DT_BF16, DT_F32 = 0, 1, 2
 _DT = {torch.float16: DT_F16, torch.bfloat16: DT_BF16, torch.float32: DT_F32}
@@ -21,37 +21,58 @@ _LAYOUT = {"half": 0, "interleaved": 1}
 PAGES = (16, 32, 64, 128)
 
 
-def _bad(where: str, what: str) -> VkbError:
-    e = VkbError(EINVAL, where)
-    e.args = (f"{where}: {what}",)
-    return e
+class _Refused(VkbError):
+    """Arguments refused before the library is called (code EINVAL)."""
+
+    def __init__(self, where: str, what: str):
+        super().__init__(EINVAL, where)
+        self.args = (f"{where}: {what}",)
 
 
-def _need(ok: bool, where: str, what: str) -> None:
-    if not ok:
-        raise _bad(where, what)
+# The current stream's handle. torch.cuda.current_stream() makes a Stream object (3 us per call on the host, as long as
+# a small launch); the handle alone is a lookup.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
+def _handle(stream, dev: int) -> int:
+    return _raw_stream(dev) if stream is None else stream.cuda_stream
+
+
+def _device(where: str, x) -> int:
+    """x's device index, which must be the current CUDA device."""
+    dev = x.get_device()
+    if dev < 0 or dev != torch.cuda.current_device():
+        raise _Refused(where, "tensors must be on the current CUDA device")
+    return dev
 
 
 def _on(stream):
     return torch.cuda.stream(stream) if stream is not None else contextlib.nullcontext()
 
 
-def _like(x, shape, dtype, stream):
-    with _on(stream):
-        return torch.empty(shape, dtype=dtype, device=x.device)
+def _made(like, stream):
+    """An output like `like`, rows adjacent, allocated for the stream of the call."""
+    if stream is None:
+        return torch.empty_like(like, memory_format=torch.contiguous_format)
+    with torch.cuda.stream(stream):
+        return torch.empty_like(like, memory_format=torch.contiguous_format)
 
 
-def _same(where: str, x, **others) -> None:
-    """Tensors of the call: on x's device, the current CUDA device."""
-    _need(x.is_cuda and x.device.index == torch.cuda.current_device(), where, "tensors must be on the current CUDA device")
-    for name, t in others.items():
-        _need(t is None or t.device == x.device, where, f"{name} must be on {x.device}")
+def _new(like, shape, dtype, stream):
+    if stream is None:
+        return like.new_empty(shape, dtype=dtype)
+    with torch.cuda.stream(stream):
+        return like.new_empty(shape, dtype=dtype)
 
 
-def _ints(where: str, x, **arrays) -> None:
-    _same(where, x, **arrays)
-    for name, t in arrays.items():
-        _need(t is None or (t.dtype == torch.int32 and t.is_contiguous()), where, f"{name} must be contiguous int32")
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+def _array(where: str, name: str, t, n: int, dtype, dev: int) -> None:
+    """t (or None) is a contiguous [n] array on the device."""
+    if t is not None and (t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or t.get_device() != dev or not t.is_contiguous()):
+        raise _Refused(where, f"{name} must be contiguous {dtype} [{n}] on the tensors' device")
 
 
 def rms_norm(x, weight, residual=None, eps: float = 1e-6, y=None, residual_out=None, q8: bool = False, stream=None):
@@ -60,31 +81,36 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6, y=None, residual_out=N
     type or None, codes or None, scales or None): with q8 also y in the Q8 format (int8 [T][d], fp16 [T][d / 32]), which
     dequant() reads. residual_out may be residual."""
     w = "rms_norm"
-    _same(w, x, weight=weight, residual=residual, y=y, residual_out=residual_out)
-    _need(x.dim() == 2 and x.dtype in _DT and (x.shape[1] == 1 or x.stride(1) == 1), w, "x must be [T][d] fp16, bf16 or fp32 with adjacent columns")
+    dt = _DT.get(x.dtype)
+    if x.dim() != 2 or dt is None or (x.shape[1] > 1 and x.stride(1) != 1):
+        raise _Refused(w, "x must be [T][d] fp16, bf16 or fp32 with adjacent columns")
     T, d = x.shape
-    _need(d > 0 and weight.dtype == x.dtype and weight.shape == (d,) and weight.is_contiguous(), w, "weight must be [d] of x's type")
-    ld = x.stride(0) if T > 1 else d
+    dev = _device(w, x)
+    if d == 0:
+        raise _Refused(w, "d must be positive")
+    _array(w, "weight", weight, d, x.dtype, dev)
     res_dt = 0
     if residual is not None:
-        _need(residual.dtype in _DT and residual.shape == x.shape and residual.is_contiguous(), w, "residual must be contiguous [T][d]")
-        res_dt = _DT[residual.dtype]
+        res_dt = _DT.get(residual.dtype)
+        if res_dt is None or residual.shape != x.shape or residual.get_device() != dev or not residual.is_contiguous():
+            raise _Refused(w, "residual must be contiguous [T][d] fp16, bf16 or fp32 on x's device")
         if residual_out is None:
-            residual_out = _like(x, (T, d), residual.dtype, stream)
-        else:
-            _need(residual_out.dtype == residual.dtype and residual_out.shape == x.shape and residual_out.is_contiguous(), w, "residual_out must be like residual")
-    else:
-        _need(residual_out is None, w, "residual_out without residual")
+            residual_out = _made(residual, stream)
+        elif residual_out.dtype != residual.dtype or residual_out.shape != x.shape or residual_out.get_device() != dev or not residual_out.is_contiguous():
+            raise _Refused(w, "residual_out must be like residual")
+    elif residual_out is not None:
+        raise _Refused(w, "residual_out without residual")
     if y is None:
-        y = _like(x, (T, d), x.dtype, stream)
-    else:
-        _need(y.dtype == x.dtype and y.shape == x.shape and y.is_contiguous(), w, "y must be contiguous [T][d] of x's type")
+        y = _made(x, stream)
+    elif y.dtype != x.dtype or y.shape != x.shape or y.get_device() != dev or not y.is_contiguous():
+        raise _Refused(w, "y must be contiguous [T][d] of x's type")
     q = s = None
     if q8:
-        _need(d % 32 == 0, w, "the Q8 output needs d % 32 == 0")
-        q, s = _like(x, (T, d), torch.int8, stream), _like(x, (T, d // 32), torch.float16, stream)
-    check(lib().vkb_rms_norm(_DT[x.dtype], x.data_ptr(), ld, _optr(residual), _optr(residual_out), res_dt, weight.data_ptr(), eps,
-                             y.data_ptr(), _optr(q), _optr(s), T, d, _stream(stream)), w)
+        if d % 32:
+            raise _Refused(w, "the Q8 output needs d % 32 == 0")
+        q, s = _new(x, (T, d), torch.int8, stream), _new(x, (T, d // 32), torch.float16, stream)
+    check(lib().vkb_rms_norm(dt, x.data_ptr(), x.stride(0) if T > 1 else d, _p(residual), _p(residual_out), res_dt,
+                             weight.data_ptr(), eps, y.data_ptr(), _p(q), _p(s), T, d, _handle(stream, dev)), w)
     return y, residual_out, q, s
 
 
@@ -98,8 +124,10 @@ def rope_turns(rot: int, base: float = 10000.0, scaling: str | None = None, fact
                   beta_slow times divided by factor, a linear ramp over the pairs between; cos and sin times
                   0.1 ln(factor) + 1"""
     w = "rope_turns"
-    _need(rot >= 2 and rot % 2 == 0, w, "rot must be even and positive")
-    _need(scaling in (None, "linear", "base", "parts") and factor >= 1.0, w, "scaling is None, linear, base or parts; factor >= 1")
+    if rot < 2 or rot % 2:
+        raise _Refused(w, "rot must be even and positive")
+    if scaling not in (None, "linear", "base", "parts") or not factor >= 1.0:
+        raise _Refused(w, "scaling is None, linear, base or parts; factor >= 1")
     n, mscale = rot // 2, 1.0
     if scaling == "base" and rot > 2:
         base = base * factor ** (rot / (rot - 2))
@@ -130,14 +158,19 @@ class KvCache:
 
     def __init__(self, k, v, k_scale, v_scale):
         w = "KvCache"
-        _need(k.dim() == 4 and k.dtype == torch.uint8 and k.is_contiguous(), w, "k must be contiguous uint8 [pages][heads][page][dim]")
-        _same(w, k, v=v, k_scale=k_scale, v_scale=v_scale)
-        _need(v.dtype == torch.uint8 and v.shape == k.shape and v.is_contiguous(), w, "v must be like k")
+        if k.dim() != 4 or k.dtype != torch.uint8 or not k.is_contiguous() or not k.is_cuda:
+            raise _Refused(w, "k must be contiguous uint8 [pages][heads][page][dim] on a CUDA device")
+        if v.dtype != torch.uint8 or v.shape != k.shape or v.device != k.device or not v.is_contiguous():
+            raise _Refused(w, "v must be like k")
         for s in (k_scale, v_scale):
-            _need(s.dtype == torch.float32 and s.shape == k.shape[:2] and s.is_contiguous(), w, "scales must be contiguous fp32 [pages][heads]")
+            if s.dtype != torch.float32 or s.shape != k.shape[:2] or s.device != k.device or not s.is_contiguous():
+                raise _Refused(w, "scales must be contiguous fp32 [pages][heads] on k's device")
         pages, self.heads, self.page, self.dim = k.shape
-        _need(self.page in PAGES, w, f"page must be one of {PAGES}")
-        _need(self.dim % 16 == 0 and 16 <= self.dim <= 256, w, "dim must be a multiple of 16 up to 256")
+        if self.page not in PAGES:
+            raise _Refused(w, f"page must be one of {PAGES}")
+        if self.dim % 16 or not 16 <= self.dim <= 256:
+            raise _Refused(w, "dim must be a multiple of 16 up to 256")
+        self.device_index = k.get_device()
         self.k, self.v, self.k_scale, self.v_scale, self.pages = k, v, k_scale, v_scale, pages
         self._s = _CacheStruct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, self.heads, self.page, self.dim)
         self._ref = ctypes.byref(self._s)
@@ -148,18 +181,24 @@ class KvCache:
         return cls(*codes, *[torch.zeros((pages, heads), dtype=torch.float32, device=device) for _ in range(2)])
 
 
-def _rows(where: str, name: str, x, heads: int, dim: int) -> int:
-    """Row stride of x [T][heads][dim] whose heads are adjacent."""
-    _need(x.dim() == 3 and x.shape[1] == heads and x.shape[2] == dim, where, f"{name} must be [T][{heads}][{dim}]")
-    _need(x.shape[0] == 0 or ((dim == 1 or x.stride(2) == 1) and (heads == 1 or x.stride(1) == dim)), where, f"{name}: the heads of a row must be adjacent")
-    return x.stride(0) if x.shape[0] > 1 else heads * dim
+def _rows(where: str, name: str, x, heads: int, dim: int, dev: int) -> int:
+    """Row stride of x [T][heads][dim], whose heads are adjacent."""
+    n, st = x.shape, x.stride()
+    if x.dim() != 3 or n[1] != heads or n[2] != dim or x.get_device() != dev or (n[0] and (st[2] != 1 or (heads > 1 and st[1] != dim))):
+        raise _Refused(where, f"{name} must be [T][{heads}][{dim}] with the heads of a row adjacent, on the cache's device")
+    return st[0] if n[0] > 1 else heads * dim
 
 
-def _batch(where: str, cache, table, lens, cu, T: int) -> int:
-    _need(table.dim() == 2 and lens.dim() == 1 and table.shape[0] == lens.shape[0] and table.shape[1] > 0, where, "table must be [B][pages], lens [B]")
-    _ints(where, cache.k, table=table, lens=lens, cu=cu)
-    B = lens.shape[0]
-    _need(B > 0 and (cu.shape == (B + 1,) if cu is not None else T == B), where, "cu must be [B + 1]; without it there is one row per sequence")
+def _batch(where: str, table, lens, cu, T: int, dev: int) -> int:
+    """The number of sequences."""
+    if table.dim() != 2 or table.dtype != torch.int32 or not table.is_contiguous() or table.get_device() != dev or not table.numel():
+        raise _Refused(where, "table must be contiguous int32 [B][pages] on the cache's device")
+    B = table.shape[0]
+    _array(where, "lens", lens, B, torch.int32, dev)
+    if cu is not None:
+        _array(where, "cu", cu, B + 1, torch.int32, dev)
+    elif T != B:
+        raise _Refused(where, "without cu there is one row per sequence")
     return B
 
 
@@ -171,47 +210,60 @@ def rope_append(cache: KvCache, table, lens, q, k, v, turns=None, cu=None, pos=N
     pos int32 [T] rotary positions (None: the place in the sequence), turns from rope_turns() (None: no rotation).
     q None: append only."""
     w = "rope_append"
-    T = k.shape[0]
-    _need(layout in _LAYOUT, w, "layout is half or interleaved")
-    _need(k.dtype in _DT and v.dtype == k.dtype, w, "k and v must be fp16, bf16 or fp32, alike")
-    ldk, ldv = _rows(w, "k", k, cache.heads, cache.dim), _rows(w, "v", v, cache.heads, cache.dim)
-    _need(v.shape[0] == T, w, "k and v must have the same rows")
-    _same(w, cache.k, k=k, v=v, q=q, q_out=q_out, turns=turns)
-    B = _batch(w, cache, table, lens, cu, T)
-    _ints(w, cache.k, pos=pos)
-    _need(pos is None or pos.shape == (T,), w, "pos must be [T]")
+    dev = _device(w, k)
+    T, heads, dim = k.shape[0], cache.heads, cache.dim
+    dt, lay = _DT.get(k.dtype), _LAYOUT.get(layout)
+    if dev != cache.device_index:
+        raise _Refused(w, "k must be on the cache's device")
+    if lay is None:
+        raise _Refused(w, "layout is half or interleaved")
+    if dt is None or v.dtype != k.dtype or v.shape != k.shape:
+        raise _Refused(w, "k and v must be fp16, bf16 or fp32, alike")
+    ldk, ldv = _rows(w, "k", k, heads, dim, dev), _rows(w, "v", v, heads, dim, dev)
+    B = _batch(w, table, lens, cu, T, dev)
+    _array(w, "pos", pos, T, torch.int32, dev)
     rot = 0
     if turns is not None:
-        _need(turns.dtype == torch.int64 and turns.dim() == 1 and turns.is_contiguous() and 2 * turns.shape[0] <= cache.dim, w, "turns must be int64 [rot / 2], rot <= dim")
         rot = 2 * turns.shape[0]
+        if rot > dim or rot == 0:
+            raise _Refused(w, "turns must be int64 [rot / 2] with 0 < rot <= dim")
+        _array(w, "turns", turns, rot // 2, torch.int64, dev)
     hq = ldq = ldo = 0
     if q is not None:
+        if q.dim() != 3 or q.shape[0] != T or q.dtype != k.dtype:
+            raise _Refused(w, "q must be [T][q_heads][dim] with k's rows and type")
         hq = q.shape[1]
-        _need(q.shape[0] == T and q.dtype == k.dtype, w, "q must have k's rows and type")
-        ldq = _rows(w, "q", q, hq, cache.dim)
+        ldq = _rows(w, "q", q, hq, dim, dev)
         if q_out is None:
-            q_out = _like(q, (T, hq, cache.dim), q.dtype, stream)
+            q_out = _made(q, stream)
+            ldo = hq * dim
         else:
-            _need(q_out.shape == q.shape and q_out.dtype == q.dtype, w, "q_out must be like q")
-        ldo = _rows(w, "q_out", q_out, hq, cache.dim)
-    else:
-        _need(q_out is None, w, "q_out without q")
-    check(lib().vkb_rope_append(cache._ref, table.data_ptr(), table.shape[1], lens.data_ptr(), _optr(cu), B, T, _DT[k.dtype],
-                                _optr(q), ldq, _optr(q_out), ldo, hq, k.data_ptr(), ldk, v.data_ptr(), ldv, _optr(pos),
-                                _optr(turns), rot, _LAYOUT[layout], mscale, _stream(stream)), w)
+            if q_out.dtype != q.dtype or q_out.shape != q.shape:
+                raise _Refused(w, "q_out must be like q")
+            ldo = _rows(w, "q_out", q_out, hq, dim, dev)
+    elif q_out is not None:
+        raise _Refused(w, "q_out without q")
+    check(lib().vkb_rope_append(cache._ref, table.data_ptr(), table.shape[1], lens.data_ptr(), _p(cu), B, T, dt,
+                                _p(q), ldq, _p(q_out), ldo, hq, k.data_ptr(), ldk, v.data_ptr(), ldv, _p(pos),
+                                _p(turns), rot, lay, mscale, _handle(stream, dev)), w)
     return q_out
 
 
 def kv_read(cache: KvCache, table, seq, pos, dtype=torch.float16, stream=None):
     """Cached tokens as values: (k, v) [n][heads][dim] of tokens pos[i] of sequences seq[i] (int32)."""
     w = "kv_read"
-    _need(table.dim() == 2 and table.shape[0] > 0 and table.shape[1] > 0, w, "table must be [B][pages]")
-    _ints(w, cache.k, table=table, seq=seq, pos=pos)
-    _need(seq.dim() == 1 and seq.shape == pos.shape and dtype in _DT, w, "seq and pos must be [n], dtype fp16, bf16 or fp32")
+    dev = _device(w, seq)
+    if dev != cache.device_index or seq.dim() != 1 or dtype not in _DT:
+        raise _Refused(w, "seq and pos must be [n] on the cache's device, dtype fp16, bf16 or fp32")
+    if table.dim() != 2 or table.dtype != torch.int32 or not table.is_contiguous() or table.get_device() != dev or not table.numel():
+        raise _Refused(w, "table must be contiguous int32 [B][pages] on the cache's device")
     n = seq.shape[0]
-    k, v = (_like(seq, (n, cache.heads, cache.dim), dtype, stream) for _ in range(2))
+    _array(w, "seq", seq, n, torch.int32, dev)
+    _array(w, "pos", pos, n, torch.int32, dev)
+    k = _new(seq, (n, cache.heads, cache.dim), dtype, stream)
+    v = _made(k, stream)
     check(lib().vkb_kv_read(cache._ref, table.data_ptr(), table.shape[1], table.shape[0], seq.data_ptr(), pos.data_ptr(), n,
-                            _DT[dtype], k.data_ptr(), v.data_ptr(), _stream(stream)), w)
+                            _DT[dtype], k.data_ptr(), v.data_ptr(), _handle(stream, dev)), w)
     return k, v
 
 
@@ -228,23 +280,31 @@ def attention(cache: KvCache, table, lens, q, cu=None, scale: float | None = Non
     only the last `window` keys up to a row's own position. work: attention_workspace() (made here when not given, at
     the cost of an allocation and a memset)."""
     w = "attention"
+    dev = _device(w, q)
+    if dev != cache.device_index or q.dim() != 3:
+        raise _Refused(w, "q must be [T][q_heads][dim] on the cache's device")
     T, hq = q.shape[0], q.shape[1]
-    _need(q.dtype in _DT, w, "q must be fp16 or bf16")
-    ldq = _rows(w, "q", q, hq, cache.dim)
-    _same(w, cache.k, q=q, out=out, work=work)
-    B = _batch(w, cache, table, lens, cu, T)
-    _need(hq > 0 and hq % cache.heads == 0, w, "q heads must be a multiple of the cache's heads")
+    if q.dtype != torch.float16 and q.dtype != torch.bfloat16:
+        raise _Refused(w, "q must be fp16 or bf16")
+    if hq == 0 or hq % cache.heads:
+        raise _Refused(w, "q heads must be a multiple of the cache's heads")
+    ldq = _rows(w, "q", q, hq, cache.dim, dev)
+    B = _batch(w, table, lens, cu, T, dev)
     if out is None:
-        out = _like(q, (T, hq, cache.dim), q.dtype, stream)
+        out = _made(q, stream)
+        ldo = hq * cache.dim
     else:
-        _need(out.shape == q.shape and out.dtype == q.dtype, w, "out must be like q")
-    ldo = _rows(w, "out", out, hq, cache.dim)
+        if out.shape != q.shape or out.dtype != q.dtype:
+            raise _Refused(w, "out must be like q")
+        ldo = _rows(w, "out", out, hq, cache.dim, dev)
     if work is None:
         with _on(stream):
             work = attention_workspace(cache)
-    check(lib().vkb_attention(cache._ref, table.data_ptr(), table.shape[1], lens.data_ptr(), _optr(cu), B, T, _DT[q.dtype],
+    elif work.get_device() != dev or not work.is_contiguous():
+        raise _Refused(w, "work must be attention_workspace()'s tensor on the cache's device")
+    check(lib().vkb_attention(cache._ref, table.data_ptr(), table.shape[1], lens.data_ptr(), _p(cu), B, T, _DT[q.dtype],
                               q.data_ptr(), ldq, out.data_ptr(), ldo, hq, cache.dim ** -0.5 if scale is None else scale,
-                              window, work.data_ptr(), work.numel() * work.element_size(), _stream(stream)), w)
+                              window, work.data_ptr(), work.numel() * work.element_size(), _handle(stream, dev)), w)
     return out
 
 
@@ -253,19 +313,24 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, toke
     temperature, top_p, min_p fp32 [B], top_k int32 [B] (None: off). Returns (token int32 [B], its probability among the
     kept tokens fp32 [B]). The rules: include/vkb.h."""
     w = "sample"
-    _need(logits.dim() == 2 and logits.dtype in _DT and logits.shape[1] > 0 and (logits.shape[1] == 1 or logits.stride(1) == 1), w, "logits must be [B][V] fp16, bf16 or fp32 with adjacent columns")
+    dt = _DT.get(logits.dtype)
+    if logits.dim() != 2 or dt is None or logits.shape[1] == 0 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise _Refused(w, "logits must be [B][V] fp16, bf16 or fp32 with adjacent columns")
     B, V = logits.shape
-    _same(w, logits, u=u, temperature=temperature, top_p=top_p, min_p=min_p, prob=prob)
-    _ints(w, logits, top_k=top_k, token=token)
-    for name, t in (("u", u), ("temperature", temperature), ("top_p", top_p), ("min_p", min_p), ("prob", prob)):
-        _need(t is None or (t.dtype == torch.float32 and t.shape == (B,) and t.is_contiguous()), w, f"{name} must be contiguous fp32 [B]")
-    for name, t in (("top_k", top_k), ("token", token)):
-        _need(t is None or t.shape == (B,), w, f"{name} must be [B]")
-    if token is None:
-        token = _like(logits, (B,), torch.int32, stream)
+    dev, f32 = _device(w, logits), torch.float32
+    _array(w, "u", u, B, f32, dev)
+    _array(w, "temperature", temperature, B, f32, dev)
+    _array(w, "top_k", top_k, B, torch.int32, dev)
+    _array(w, "top_p", top_p, B, f32, dev)
+    _array(w, "min_p", min_p, B, f32, dev)
     if prob is None:
-        prob = _like(logits, (B,), torch.float32, stream)
-    check(lib().vkb_sample(_DT[logits.dtype], logits.data_ptr(), logits.stride(0) if B > 1 else V, B, V, _optr(temperature),
-                           _optr(top_k), _optr(top_p), _optr(min_p), u.data_ptr(), token.data_ptr(), prob.data_ptr(),
-                           _stream(stream)), w)
+        prob = _made(u, stream)
+    else:
+        _array(w, "prob", prob, B, f32, dev)
+    if token is None:
+        token = _new(u, (B,), torch.int32, stream)
+    else:
+        _array(w, "token", token, B, torch.int32, dev)
+    check(lib().vkb_sample(dt, logits.data_ptr(), logits.stride(0) if B > 1 else V, B, V, _p(temperature), _p(top_k), _p(top_p),
+                           _p(min_p), u.data_ptr(), token.data_ptr(), prob.data_ptr(), _handle(stream, dev)), w)
     return token, prob
