@@ -70,6 +70,80 @@ __device__ __forceinline__ float ex2_ftz(float x) {
     return r;
 }
 
+// Pairs of floats (one register pair, one instruction per operation).
+__device__ __forceinline__ uint64_t f2_make(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 f2_get(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t x, uint64_t y, uint64_t z) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t x, uint64_t y) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+
+// Maximum of x = s kf + lv over 32 scores (two groups of 16 keys, the first at key k0); MASK: keys outside [klo, khi) out.
+template <bool MASK>
+__device__ __forceinline__ float pr_max(const uint32_t (&s)[32], const float4* sc, float qinv, int k0, int klo, int khi,
+                                        float mx) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            float v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[i] = __uint_as_float(s[16 * h + e + i]);
+                if (MASK && (k0 + 16 * h + e + i < klo || k0 + 16 * h + e + i >= khi)) v[i] = -INFINITY;
+            }
+            m0 = fmaxf(fmaxf(m0, v[0]), v[1]);
+            m1 = fmaxf(fmaxf(m1, v[2]), v[3]);
+        }
+        const float m = fmaxf(m0, m1);
+        const float4 f = sc[h];
+        if (!MASK || m > -INFINITY) mx = fmaxf(mx, fmaf(m, f.x * qinv, f.y));
+    }
+    return mx;
+}
+// p' of 32 scores as fp16 pairs, and their sum into l (two running halves).
+template <bool MASK>
+__device__ __forceinline__ void pr_exp(const uint32_t (&s)[32], uint32_t (&pk)[16], const float4* sc, float qinv, float mb,
+                                       int k0, int klo, int khi, uint64_t& l) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const float4 f = sc[h];
+        const float kf = f.x * qinv, cg = f.y - mb;
+        const uint64_t kf2 = f2_make(kf, kf), cg2 = f2_make(cg, cg);
+        uint64_t sum = 0;
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+            float2 x = f2_get(f2_fma(f2_make(__uint_as_float(s[16 * h + e]), __uint_as_float(s[16 * h + e + 1])), kf2, cg2));
+            if (MASK) {
+                const int k = k0 + 16 * h + e;
+                if (k < klo || k >= khi) x.x = -INFINITY;
+                if (k + 1 < klo || k + 1 >= khi) x.y = -INFINITY;
+            }
+            x.x = ex2_ftz(x.x);
+            x.y = ex2_ftz(x.y);
+            const uint64_t p = f2_make(x.x, x.y);
+            sum = e == 0 ? p : f2_add(sum, p);
+            pk[8 * h + e / 2] = pack_f16(x.x, x.y);
+        }
+        l = f2_fma(sum, f2_make(f.z, f.z), l);
+    }
+}
+
 // 32 lanes x 16 consecutive columns from registers (no wait: tmem_wait_st).
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile(
@@ -189,9 +263,6 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
             }
             jj += n;
         }
-        // every commit of this block has arrived before tensor memory is freed
-        if (ok && jj > 0)
-            for (int t = 0; t < NT; ++t) wait(&o_full[t], jj - 1);
     } else if (warp >= 16 - C::ND / 32) {
         // ===================== convert codes =====================
         constexpr int CPR = DT / 16, EACH = PR_KT * CPR / C::ND;   // 16-code chunks per row; per thread and tile
@@ -345,7 +416,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
             const float qinv = bf && n > 0 ? __fdiv_rn(1.f, rowf[r]) : 1.f;
             const int all_hi = g.pos0 + g.r0 / a.G + 1;   // keys [all_lo, all_hi): every row of the item sees them
             const int all_lo = a.window > 0 ? g.pos0 + (g.r0 + g.rows - 1) / a.G - a.window + 1 : 0;
-            float M = -INFINITY, l = 0.f, vs0 = 0.f;
+            float M = -INFINITY, vs0 = 0.f;
+            uint64_t l2 = 0;   // the sum of p, two halves
             for (int j = 0; j < n; ++j) {
                 const int J = jj + j, buf = NT == 2 ? t : J & 1, key0 = (g.t0 + j) * PR_KT;
                 if (ok) ok = __all_sync(0xffffffffu, wait_parity_sleep(&s_full[buf], (NT == 2 ? J : J >> 1) & 1));
@@ -356,34 +428,31 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
                 const uint32_t ts = tl + buf * 128;
                 const bool masked = key0 + PR_KT > all_hi || key0 < all_lo || r >= g.rows;
                 const bool wmask = __any_sync(0xffffffffu, masked);
-                uint32_t s[32];
+                uint32_t s[32], s2[32];   // 32 scores each: one chunk is worked on while the next one is read
                 // ---- maximum of x ----
                 float mx = -INFINITY;
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    tmem_ld32(ts + 32 * c, s);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        float m = -INFINITY;
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            float v = __uint_as_float(s[16 * h + e]);
-                            if (wmask) {
-                                const int k = key0 + 32 * c + 16 * h + e;
-                                if (k < klo || k >= khi) v = -INFINITY;
-                            }
-                            m = fmaxf(m, v);
-                        }
-                        const float4 f = sc[2 * c + h];
-                        if (m > -INFINITY) mx = fmaxf(mx, fmaf(m, f.x * qinv, f.y));
-                    }
-                }
+                auto max_of = [&](const uint32_t (&v)[32], int c) {
+                    mx = wmask ? pr_max<true>(v, sc + 2 * c, qinv, key0 + 32 * c, klo, khi, mx)
+                               : pr_max<false>(v, sc + 2 * c, qinv, 0, 0, 0, mx);
+                };
+                tmem_ld32_async(ts, s);
+                tmem_wait_ld(s);
+                tmem_ld32_async(ts + 32, s2);
+                max_of(s, 0);
+                tmem_wait_ld(s2);
+                tmem_ld32_async(ts + 64, s);
+                max_of(s2, 1);
+                tmem_wait_ld(s);
+                tmem_ld32_async(ts + 96, s2);
+                max_of(s, 2);
+                tmem_wait_ld(s2);
+                max_of(s2, 3);
                 vs0 = sc[0].w;
                 const bool grow = mx > M + PR_LAZY || (mx > -INFINITY && M == -INFINITY);
                 if (__any_sync(0xffffffffu, grow)) {
                     const float mn = fmaxf(M, mx), al = M == -INFINITY ? 0.f : ex2_ftz(M - mn);
                     M = mn;
-                    l *= al;
+                    l2 = f2_fma(l2, f2_make(al, al), 0);
                     if (j > 0) {   // O of the tiles before this one, once its last MMA is done
                         if (ok) ok = __all_sync(0xffffffffu, wait_parity_sleep(&o_full[t], (J - 1) & 1));
                         tc_fence_after();
@@ -397,42 +466,37 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
                         }
                     }
                 }
-                // ---- p' and its sum ----
+                // ---- p' and its sum. P's columns 16 c .. 16 c + 15 lie in S's columns below 32 c + 32, which have been
+                // read ----
                 const float mb = M == -INFINITY ? 0.f : M - PR_BIAS;
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    tmem_ld32(ts + 32 * c, s);
+                auto exp_of = [&](const uint32_t (&v)[32], int c) {
                     uint32_t pk[16];
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float4 f = sc[2 * c + h];
-                        const float kf = f.x * qinv, cg = f.y - mb;
-                        float sum0 = 0.f, sum1 = 0.f;
-#pragma unroll
-                        for (int e = 0; e < 16; e += 2) {
-                            float x0 = fmaf(__uint_as_float(s[16 * h + e]), kf, cg);
-                            float x1 = fmaf(__uint_as_float(s[16 * h + e + 1]), kf, cg);
-                            if (wmask) {
-                                const int k = key0 + 32 * c + 16 * h + e;
-                                if (k < klo || k >= khi) x0 = -INFINITY;
-                                if (k + 1 < klo || k + 1 >= khi) x1 = -INFINITY;
-                            }
-                            const float p0 = ex2_ftz(x0), p1 = ex2_ftz(x1);
-                            sum0 += p0;
-                            sum1 += p1;
-                            pk[8 * h + e / 2] = pack_f16(p0, p1);
-                        }
-                        l = fmaf(sum0 + sum1, f.z, l);
-                    }
-                    // P's columns 16 c .. 16 c + 15 lie in S's columns below 32 c + 32, which have been read
+                    if (wmask) pr_exp<true>(v, pk, sc + 2 * c, qinv, mb, key0 + 32 * c, klo, khi, l2);
+                    else pr_exp<false>(v, pk, sc + 2 * c, qinv, mb, 0, 0, 0, l2);
                     tmem_st16(ts + 16 * c, pk);
-                }
+                };
+                tmem_ld32_async(ts, s);
+                tmem_wait_ld(s);
+                tmem_ld32_async(ts + 32, s2);
+                exp_of(s, 0);
+                tmem_wait_ld(s2);
+                tmem_ld32_async(ts + 64, s);
+                exp_of(s2, 1);
+                tmem_wait_ld(s);
+                tmem_ld32_async(ts + 96, s2);
+                exp_of(s, 2);
+                tmem_wait_ld(s2);
+                exp_of(s2, 3);
                 tmem_wait_st();
+                // A barrier's phase can be waited for only until the next one completes: with one row tile this tile's S
+                // does not follow from the last O update, so every update is waited for, before this P allows the next
+                if (NT == 1 && j > 0 && ok) ok = __all_sync(0xffffffffu, wait_parity_sleep(&o_full[t], (J - 1) & 1));
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[buf]);
             }
             // ---- the item's part, or its output ----
+            const float l = f2_get(l2).x + f2_get(l2).y;
             if (n > 0 && ok) ok = __all_sync(0xffffffffu, wait_parity_sleep(&o_full[t], (jj + n - 1) & 1));
             tc_fence_after();
             const uint32_t to = tl + C::o_col + t * DT;
@@ -467,6 +531,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
             if (!g.whole) attn_join<DT, C::ROWS, T>(a, run, g, stid, nsm, join_sh, bar);
         }
     }
+    // The softmax warps have waited for the last O update, and so for every MMA, before tensor memory is freed
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
