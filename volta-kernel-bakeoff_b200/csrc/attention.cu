@@ -49,6 +49,10 @@ static int launch_prompt(const vkb_kv_cache_t* c, const AttnArgs& a, int dev, cu
     static cudaError_t err[kMaxDevices];
     std::call_once(once[dev], [&] {
         err[dev] = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::BYTES);
+        // the kernel's register split needs the registers that the block is launched with
+        cudaFuncAttributes fa;
+        if (err[dev] == cudaSuccess) err[dev] = cudaFuncGetAttributes(&fa, kern);
+        if (err[dev] == cudaSuccess && fa.numRegs != 128) err[dev] = cudaErrorInvalidConfiguration;
     });
     if (err[dev] != cudaSuccess) return -(int)err[dev];
     return launch_pdl(kern, dim3((unsigned)device_info(dev).sm_count), dim3(PR_THREADS), C::BYTES, st, 1, a,

@@ -25,7 +25,7 @@ struct AttnArgs {
     const float* vs;
     const void* q;
     void* out;
-    float* part;          // [grid][2][ROWS][DT + 2]
+    float* part;          // [grid][2] parts: sums [DT / 4][ROWS][4], then {maximum, sum} [ROWS][2]
     unsigned* cnt;        // [grid] arrivals of the item that starts in this block; zero between calls
     long long ldq, ldo;
     float scale_log2;     // scale * log2(e)
@@ -229,38 +229,36 @@ __device__ __forceinline__ void attn_join(const AttnArgs& a, const AttnRun& r, c
     bar();
     if (!*sh) return;
     constexpr int PITCH = DT + 2;
-    const int per = a.dim >> 2;   // a thread takes four columns of a row
     const float* base = a.part;
     auto slot = [&](int c) { return base + (2ll * c + (c == c0 ? 1 : 0)) * ROWS * PITCH; };
-    for (int i = tid; i < g.rows * per; i += n) {
-        const int row = i / per, d = 4 * (i - row * per);
+    // A thread takes four columns of a row; neighbouring threads neighbouring rows, as the parts lie.
+    const int work = g.rows * (a.dim >> 2);
+    for (int i = tid; i < work; i += n) {
+        const int d4 = i / g.rows, row = i - d4 * g.rows;
         float m = -INFINITY;
 #pragma unroll 8
         for (int c = c0; c <= c1; ++c) m = fmaxf(m, __ldcg(slot(c) + ROWS * DT + 2 * row));
+        if (m == -INFINITY) m = 0.f;   // no part saw a key
         float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-        if (m > -INFINITY || m != m) {
-#pragma unroll 4
-            for (int c = c0; c <= c1; ++c) {
-                const float* p = slot(c);
-                const float2 ml = __ldcg(reinterpret_cast<const float2*>(p + ROWS * DT + 2 * row));
-                const float4 v = __ldcg(reinterpret_cast<const float4*>(p + row * DT + d));
-                const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);
-                l = fmaf(w, ml.y, l);
-                o[0] = fmaf(w, v.x, o[0]);
-                o[1] = fmaf(w, v.y, o[1]);
-                o[2] = fmaf(w, v.z, o[2]);
-                o[3] = fmaf(w, v.w, o[3]);
-            }
+#pragma unroll 8
+        for (int c = c0; c <= c1; ++c) {
+            const float* p = slot(c);
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p + ROWS * DT + 2 * row));
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(p) + d4 * ROWS + row);
+            const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);
+            l = fmaf(w, ml.y, l);
+            o[0] = fmaf(w, v.x, o[0]);
+            o[1] = fmaf(w, v.y, o[1]);
+            o[2] = fmaf(w, v.z, o[2]);
+            o[3] = fmaf(w, v.w, o[3]);
         }
         const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
-        T* out = attn_out<T>(a, g, row) + d;
-        uint32_t w01, w23;
-        if constexpr (sizeof(T) == 2) {
-            constexpr bool half = std::is_same<T, __half>::value;
-            w01 = half ? pack_f16(o[0] * inv, o[1] * inv) : pack_bf16(o[0] * inv, o[1] * inv);
-            w23 = half ? pack_f16(o[2] * inv, o[3] * inv) : pack_bf16(o[2] * inv, o[3] * inv);
-            *reinterpret_cast<uint2*>(out) = make_uint2(w01, w23);
-        }
+        uint2 w;
+        if constexpr (std::is_same<T, __half>::value)
+            w = make_uint2(pack_f16(o[0] * inv, o[1] * inv), pack_f16(o[2] * inv, o[3] * inv));
+        else
+            w = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
+        *reinterpret_cast<uint2*>(attn_out<T>(a, g, row) + 4 * d4) = w;
     }
 }
 

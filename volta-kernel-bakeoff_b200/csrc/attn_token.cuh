@@ -430,7 +430,7 @@ attn_token_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
                             *reinterpret_cast<uint32_t*>(out) =
                                 std::is_same<T, __half>::value ? pack_f16(v.x, v.y) : pack_bf16(v.x, v.y);
                         } else {
-                            *reinterpret_cast<float2*>(part + r * DT + 32 * c + d) = v;
+                            *reinterpret_cast<float2*>(part + ((8 * c + (d >> 2)) * C::ROWS + r) * 4 + (d & 3)) = v;
                         }
                     }
                 }
