@@ -18,10 +18,10 @@ static size_t attn_part_floats(int dt) {
     return (size_t)(dt == 256 ? 128 : 256) * (dt + 2);   // the prompt kernel's tile is the larger one
 }
 
-template <int DT, int MT, typename T>
+template <int DT, int NQ, typename T>
 static int launch_token(const vkb_kv_cache_t* c, const AttnArgs& a, int dev, cudaStream_t st) {
-    using C = TkCfg<DT, MT>;
-    auto kern = attn_token_kernel<DT, MT, T>;
+    using C = TkCfg<DT, NQ>;
+    auto kern = attn_token_kernel<DT, NQ, T>;
     static std::once_flag once[kMaxDevices];
     static cudaError_t err[kMaxDevices];
     std::call_once(once[dev], [&] {
@@ -29,7 +29,7 @@ static int launch_token(const vkb_kv_cache_t* c, const AttnArgs& a, int dev, cud
         // the kernel's register split needs the registers that the block is launched with
         cudaFuncAttributes fa;
         if (err[dev] == cudaSuccess) err[dev] = cudaFuncGetAttributes(&fa, kern);
-        if (err[dev] == cudaSuccess && fa.numRegs * TK_THREADS < 128 * 40 + 256 * 232) err[dev] = cudaErrorInvalidConfiguration;
+        if (err[dev] == cudaSuccess && fa.numRegs < C::LREG) err[dev] = cudaErrorInvalidConfiguration;
     });
     if (err[dev] != cudaSuccess) return -(int)err[dev];
     CUtensorMap tk, tv;
@@ -38,7 +38,7 @@ static int launch_token(const vkb_kv_cache_t* c, const AttnArgs& a, int dev, cud
     const CUtensorMapSwizzle swz = DT == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
     if (int r = get_tmap_2d(&tk, c->k, rows, c->dim, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, C::HB, pb, swz)) return r;
     if (int r = get_tmap_2d(&tv, c->v, rows, c->dim, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, C::HB, pb, swz)) return r;
-    return launch_pdl(kern, dim3((unsigned)device_info(dev).sm_count), dim3(TK_THREADS), C::BYTES, st, 1, tk, tv, a);
+    return launch_pdl(kern, dim3((unsigned)device_info(dev).sm_count), dim3(C::THREADS), C::BYTES, st, 1, tk, tv, a);
 }
 
 template <int DT, typename T>
@@ -61,22 +61,21 @@ static int launch_prompt(const vkb_kv_cache_t* c, const AttnArgs& a, int dev, cu
 
 template <typename T>
 static int attn_dispatch(const vkb_kv_cache_t* c, const AttnArgs& a, int dev, cudaStream_t st) {
-    // Query rows per sequence and kv head, on average: the row tile that holds them (a tile of 16 rows per product).
+    // Query rows per sequence and kv head, on average: the smallest tile of the token kernel that holds them; the prompt
+    // kernel where they are more than its largest.
     const long long rows = ((long long)a.T + a.B - 1) / a.B * a.G;
-    if (rows > 64) {
-        switch (attn_dt(c->dim)) {
-            case 64: return launch_prompt<64, T>(c, a, dev, st);
-            case 128: return launch_prompt<128, T>(c, a, dev, st);
-            default: return launch_prompt<256, T>(c, a, dev, st);
-        }
-    }
     switch (attn_dt(c->dim)) {
         case 64:
-            return rows <= 16 ? launch_token<64, 1, T>(c, a, dev, st)
-                   : rows <= 32 ? launch_token<64, 2, T>(c, a, dev, st) : launch_token<64, 4, T>(c, a, dev, st);
+            return rows <= 8    ? launch_token<64, 1, T>(c, a, dev, st)
+                   : rows <= 16 ? launch_token<64, 2, T>(c, a, dev, st)
+                   : rows <= 32 ? launch_token<64, 4, T>(c, a, dev, st) : launch_prompt<64, T>(c, a, dev, st);
         case 128:
-            return rows <= 16 ? launch_token<128, 1, T>(c, a, dev, st) : launch_token<128, 2, T>(c, a, dev, st);
-        default: return launch_token<256, 1, T>(c, a, dev, st);
+            return rows <= 8    ? launch_token<128, 1, T>(c, a, dev, st)
+                   : rows <= 16 ? launch_token<128, 2, T>(c, a, dev, st)
+                   : rows <= 32 ? launch_token<128, 4, T>(c, a, dev, st) : launch_prompt<128, T>(c, a, dev, st);
+        default:
+            return rows <= 8    ? launch_token<256, 1, T>(c, a, dev, st)
+                   : rows <= 16 ? launch_token<256, 2, T>(c, a, dev, st) : launch_prompt<256, T>(c, a, dev, st);
     }
 }
 

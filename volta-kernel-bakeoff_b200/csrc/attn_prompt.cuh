@@ -22,7 +22,7 @@
 //                 (K: K-major B operand; V: the same bytes are the MN-major B operand of P V)
 #pragma once
 
-#include "attn_common.cuh"
+#include "attn_token.cuh"
 #include "tcgen05.cuh"
 
 namespace vkb {
@@ -82,18 +82,6 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint3
         : "memory");
 }
 
-__device__ __forceinline__ float ex2_ftz(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-
-// Larger of fp16 pairs; a NaN stays.
-__device__ __forceinline__ uint32_t h2_max(uint32_t x, uint32_t y) {
-    uint32_t r;
-    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
-    return r;
-}
 // Pairs of floats (one register pair, one instruction per operation).
 __device__ __forceinline__ uint64_t f2_make(float x, float y) {
     uint64_t r;
@@ -153,8 +141,8 @@ __device__ __forceinline__ void pr_exp(const uint32_t (&s)[32], uint32_t (&pk)[1
 #pragma unroll
         for (int e = 0; e < 16; e += 2) {
             float2 x = f2_get(f2_fma(f2_make(__uint_as_float(s[16 * h + e]), __uint_as_float(s[16 * h + e + 1])), kf2, cg2));
-            x.x = ex2_ftz(x.x);
-            x.y = ex2_ftz(x.y);
+            x.x = ex2(x.x);
+            x.y = ex2(x.y);
             const uint64_t p = f2_make(x.x, x.y);
             sum[(e >> 1) & 1] = e < 4 ? p : f2_add(sum[(e >> 1) & 1], p);
             pk[8 * h + e / 2] = pack_f16(x.x, x.y);
@@ -456,8 +444,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
                             for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(f[e]));
 #pragma unroll
                             for (int o = LPR / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                            const int e2 = (int)(__float_as_uint(m) >> 23) - 127;
-                            const float fac = m == 0.f ? 1.f : exp2f((float)min(126, max(-126, 13 - e2)));
+                            const float fac = row_factor(m);
                             if (c == 0) rowf[128 * t + rl] = fac;
                             v[i] = make_uint4(pack_f16(f[0] * fac, f[1] * fac), pack_f16(f[2] * fac, f[3] * fac),
                                               pack_f16(f[4] * fac, f[5] * fac), pack_f16(f[6] * fac, f[7] * fac));
@@ -518,7 +505,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
                 const bool unset = M == -INFINITY && klo < key0 + PR_KT && khi > key0;   // the row's first keys
                 if (__any_sync(0xffffffffu, unset || (top & 0xffffu) > 0x6c00u || (top >> 16) > 0x6c00u)) {
                     const float mx = pr_max(s2, sc + 2, qinv, pr_max(s, sc, qinv, -INFINITY));
-                    const float mn = fmaxf(M, mx), al = M == -INFINITY ? 0.f : ex2_ftz(M - mn);
+                    const float mn = fmaxf(M, mx), al = M == -INFINITY ? 0.f : ex2(M - mn);
                     M = mn;
                     l2 = f2_fma(l2, f2_make(al, al), 0);
                     if (j > 0) {   // O of the tiles before this one, once its last MMA is done

@@ -1,18 +1,22 @@
 // Attention for few query rows per kv head (single tokens, drafted tokens): HBM-bound, the codes are read once and
 // everything else hides behind that stream.
 //
-//   s_rj = (q_r . c_j) ks_j scale, p_rj = exp(s_rj - m_r), o_r = sum_j p_rj vs_j c'_j / sum_j p_rj
+//   s_jr = (c_j . q_r) ks_j scale log2(e),  p'_jr = 2^(s_jr + log2(vs_j / V) - M_r + 8),
+//   O'_r = sum_j p'_jr c'_j,   l_r = sum_j p'_jr (V / vs_j),   o_r = V O'_r / l_r
 //
-// with codes c, c' and one scale per page for K (ks) and V (vs). One persistent block per SM (its run of units:
-// attn_common.cuh), three warpgroups. Warp 8 streams: per unit of 64 keys, one TMA box of codes per page piece and 128-byte
-// half for K and for V (128-byte swizzle), and the pages' scales with 4-byte asynchronous copies, into a ring of NS
-// stages. Warps 0-3 compute the even units, warps 4-7 the odd ones, 16 keys per warp, each warp with its own running
-// maximum and sum, joined once per segment. Products are mma.sync.m16n8k16 on fp16: the codes enter exactly (1024 + u as
-// fp16, minus 1152), K through ldmatrix and V through transposing ldmatrix on byte pairs, so a register of four codes
-// is one operand register pair either way; the scales are applied in fp32 (K) and folded into p before its one
-// rounding to fp16 (V). tcgen05 has nothing to add here: with 16 rows the tensor work is an eighth of the time.
-// p carries a factor 2^8 and the running maximum follows the true one lazily (by up to 2^4), so small p keep their
-// fp16 precision: the smallest normal p is 2^-22 of the largest.
+// with codes c, c', one scale per page for K (ks) and V (vs), and V the largest vs so far. One persistent block per SM
+// (its run of units: attn_common.cuh), computing warps and a streaming one. The streaming warp brings, per unit of 64
+// keys, one TMA box of codes per page piece and 128-byte half for K and for V (128-byte swizzle), and the pages' scales
+// with 4-byte asynchronous copies, into a ring of NS stages. Groups of four computing warps take the units in turn, 16
+// keys per warp, each warp with its own M and sums, joined once per segment.
+// Products are mma.sync.m16n8k16 on fp16 with the keys (or the dimensions) as the 16 rows and the queries as the 8
+// columns: S^T = C q^T, then O^T += C'^T p^T, so that 8 query rows (a kv head's q heads) fill a tile; as the 16 rows of
+// q C^T they left three quarters of it empty (470 instead of 260 instructions per 16 keys, 193 us at 64 sequences of
+// up to 8192 tokens). The codes enter exactly (1024 + u as fp16, minus 1152), K through ldmatrix and V through
+// transposing ldmatrix on byte pairs, so that a register of four codes gives two operand registers either way; p^T
+// reaches the second product through movmatrix. tcgen05 has nothing to add: with 8 rows its tiles would be empty.
+// p' is rounded once, to fp16, for the product. It is computed against the M of the keys before; only where one passes
+// 2^(8 + 4) the warp finds the new maximum, rescales and computes it again. vs below 2^-30 V counts as that.
 // q: fp16 as it is; bf16 rows are scaled by a power of two into fp16's range first (exact but for values 2^-28 below the
 // row's largest).
 #pragma once
@@ -22,29 +26,34 @@
 namespace vkb {
 
 constexpr int AT_KT = 64;                            // keys per unit
-constexpr int TK_WARPS = 8;                          // computing warps (two groups of four)
-constexpr int TK_THREADS = 32 * (TK_WARPS + 4);      // and a warpgroup whose first warp streams
-constexpr float TK_P_BIAS = 8.f;                     // p is kept times 2^8
-constexpr float TK_LAZY = 4.f;                       // the reference maximum may lag the true one by 2^4
+constexpr float TK_P_BIAS = 8.f;                     // p' is kept times 2^8
 
-// DT: head dimension rounded up to 64, 128 or 256. MT: 16-row tiles per item.
-template <int DT, int MT> struct TkCfg {
-    static constexpr int ROWS = 16 * MT;
+// DT: head dimension rounded up to 64, 128 or 256. NQ: tiles of 8 query rows per item.
+template <int DT, int NQ> struct TkCfg {
+    static constexpr int ROWS = 8 * NQ;
+    static constexpr int OREG = DT * NQ / 4;                  // accumulator registers of a thread
+    static constexpr int WARPS = OREG <= 32 ? 16 : 8;         // computing warps (groups of four)
+    static constexpr int GROUPS = WARPS / 4;
+    static constexpr int THREADS = 32 * (WARPS + 4);          // and a warpgroup whose first warp streams
+    // registers: launched with LREG per thread; the streaming warpgroup keeps PREG, the computing ones have CREG
+    static constexpr int LREG = WARPS == 16 ? 96 : 168, PREG = WARPS == 16 ? 32 : 40, CREG = WARPS == 16 ? 112 : 232;
+    static_assert(128 * PREG + 32 * WARPS * CREG <= THREADS * LREG, "the split is of what the block is launched with");
+    static constexpr bool QREGS = NQ == 1 && DT <= 128;       // q fragments in registers
     static constexpr int HB = DT < 128 ? DT : 128;            // bytes of a box row
     static constexpr int TILE = AT_KT * DT;                   // bytes of one tensor's codes in a stage
     static constexpr int STAGE = 2 * TILE;
-    static constexpr int NS = DT == 64 ? 12 : DT == 128 ? 8 : 5;
-    static constexpr int Q = ROWS * DT * 2;                   // q in A-fragment order
-    static constexpr int MERGE = TK_WARPS * 16 * 32 * 4;      // 32 columns of 16 rows of every warp
+    static constexpr int NS = DT == 64 ? 16 : DT == 128 ? 10 : 5;
+    static constexpr int Q = QREGS ? 0 : ROWS * DT * 2;       // q in B-fragment order
+    static constexpr int MERGE = WARPS * 8 * 64 * 4;          // 64 columns of 8 rows of every warp
     // offsets from the 1024-aligned base
     static constexpr int q_off = NS * STAGE;
     static constexpr int merge_off = q_off + Q;
-    static constexpr int ml_off = merge_off + MERGE;          // [warp][ROWS] {m, l}
-    static constexpr int row_off = ml_off + TK_WARPS * ROWS * 8;   // [ROWS] factor of q
+    static constexpr int ml_off = merge_off + MERGE;          // [warp][ROWS] {M, l}
+    static constexpr int row_off = ml_off + WARPS * ROWS * 8; // [ROWS] factor of q
     static constexpr int sc_off = row_off + ROWS * 4;         // [NS][4 pieces]{k, v} scales
     static constexpr int bar_off = (sc_off + NS * 32 + 15) / 16 * 16;
     static constexpr int run_off = bar_off + 16 * NS;
-    static constexpr int BYTES = run_off + 8 * (TK_THREADS / 32 + 2) + 16 + 1024;
+    static constexpr int BYTES = run_off + 8 * (THREADS / 32 + 2) + 16 + 1024;
 };
 
 __device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
@@ -59,6 +68,19 @@ __device__ __forceinline__ void ldsm_x4_t(uint32_t (&r)[4], uint32_t addr) {
                  : "r"(addr)
                  : "memory");
 }
+// The transpose of an 8 x 8 matrix of 16-bit elements, one row's neighbouring pair per thread.
+__device__ __forceinline__ uint32_t movm(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+// D += A B without volatile: the compiler may interleave independent products.
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 // Bytes (i, j) of v (codes + 128) as the exact fp16 pair of codes: 0x6400 | u is 1024 + u, minus 1152.
 __device__ __forceinline__ uint32_t codes_f16(uint32_t v, uint32_t sel) {
     return h2_sub(prmt(v, 0x64646464u, sel), 0x64806480u);
@@ -68,6 +90,17 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+// Larger of fp16 pairs; a NaN stays.
+__device__ __forceinline__ uint32_t h2_max(uint32_t x, uint32_t y) {
+    uint32_t r;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
+    return r;
+}
+// The power of two that brings a row of largest magnitude m into [2^13, 2^14).
+__device__ __forceinline__ float row_factor(float m) {
+    const int e = (int)(__float_as_uint(m) >> 23) - 127;             // floor(log2 m); tiny: -127
+    return m == 0.f ? 1.f : exp2f((float)min(126, max(-126, 13 - e)));
+}
 
 // Shared address of 16-byte chunk c of key row r of a stage's tile of codes (the TMA swizzles: 128-byte rows XOR the row's
 // low three bits into the chunk, 64-byte rows bits 1-2 of the row).
@@ -76,39 +109,69 @@ template <int DT> __device__ __forceinline__ uint32_t code_addr(uint32_t tile, i
     else return tile + (c >> 3) * (AT_KT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
 
-template <int DT, int MT, typename T>
-__global__ void __launch_bounds__(TK_THREADS, 1)
+// The B fragments of query row tile nq of a segment: {b0, b1} of k step ks hold elements 16 ks + 4 c .. + 3 of query
+// 8 nq + lane / 4, the k order of the codes' registers. Returns the row's factor (bf16).
+template <int DT, typename T>
+__device__ __forceinline__ float tk_load_q(const AttnArgs& a, const AttnSeg& g, int nq, int lane, uint2 (&w)[DT / 16]) {
+    const int r = 8 * nq + (lane >> 2), qc = lane & 3;
+    const bool on = r < g.rows;
+    const int t = (g.r0 + (on ? r : 0)) / a.G, hq = g.h * a.G + (g.r0 + (on ? r : 0)) - t * a.G;
+    const T* q = reinterpret_cast<const T*>(a.q) + (g.q0 + t) * a.ldq + (long long)hq * a.dim + 4 * qc;
+#pragma unroll
+    for (int ks = 0; ks < DT / 16; ++ks) {
+        w[ks] = make_uint2(0u, 0u);
+        if (on && 16 * ks < a.dim) w[ks] = *reinterpret_cast<const uint2*>(q + 16 * ks);
+    }
+    float f = 1.f;
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        float m = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < DT / 16; ++ks)
+            m = fmaxf(m, fmaxf(fmaxf(fabsf(__uint_as_float(w[ks].x << 16)), fabsf(__uint_as_float(w[ks].x & 0xffff0000u))),
+                               fmaxf(fabsf(__uint_as_float(w[ks].y << 16)), fabsf(__uint_as_float(w[ks].y & 0xffff0000u)))));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        f = row_factor(m);
+#pragma unroll
+        for (int ks = 0; ks < DT / 16; ++ks) {
+            w[ks].x = pack_f16(__uint_as_float(w[ks].x << 16) * f, __uint_as_float(w[ks].x & 0xffff0000u) * f);
+            w[ks].y = pack_f16(__uint_as_float(w[ks].y << 16) * f, __uint_as_float(w[ks].y & 0xffff0000u) * f);
+        }
+    }
+    return f;
+}
+
+template <int DT, int NQ, typename T>
+__global__ void __launch_bounds__(TkCfg<DT, NQ>::THREADS, 1)
 attn_token_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                   const __grid_constant__ AttnArgs a) {
-    using C = TkCfg<DT, MT>;
+    using C = TkCfg<DT, NQ>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint64_t* full = reinterpret_cast<uint64_t*>(sm + C::bar_off);
     uint64_t* empty = full + C::NS;
     float* scales = reinterpret_cast<float*>(sm + C::sc_off);
     long long* run_sh = reinterpret_cast<long long*>(sm + C::run_off);
-    volatile int* join_sh = reinterpret_cast<volatile int*>(run_sh + TK_THREADS / 32 + 2);
+    volatile int* join_sh = reinterpret_cast<volatile int*>(run_sh + C::THREADS / 32 + 2);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     pdl_trigger();
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::NS; ++i) {
             mbar_init(&full[i], 1 + 32);   // the boxes' bytes, and the 32 lanes' scale copies
-            mbar_init(&empty[i], TK_WARPS / 2);
+            mbar_init(&empty[i], 4);
         }
         fence_mbar_init();
         prefetch_tmap(&tk);
         prefetch_tmap(&tv);
     }
     pdl_wait();
-    AttnRun run = attn_run<C::ROWS, AT_KT, TK_THREADS>(a, run_sh);   // its barriers also publish the mbarriers
+    AttnRun run = attn_run<C::ROWS, AT_KT, C::THREADS>(a, run_sh);   // its barriers also publish the mbarriers
     AttnSeg g;
 
-    // Registers: 384 threads are launched with 168 each (64512); the streaming warpgroup keeps 40, so that the computing
-    // ones have 232 (128 x 40 + 256 x 232 = 64512).
-    if (warp >= TK_WARPS) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-        if (warp > TK_WARPS) return;
+    if (warp >= C::WARPS) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::PREG));
+        if (warp > C::WARPS) return;
         // ===================== producer =====================
         const int pb = min(AT_KT, 1 << a.page_log2);   // keys per box
         int it = 0;
@@ -161,10 +224,12 @@ attn_token_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     }
 
     // ===================== computing warps =====================
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
-    const int grp = warp >> 2, wk = (warp & 3) * 16;   // unit parity, first key of the unit that this warp takes
-    const int gr = lane >> 2, qc = lane & 3;           // fragment row and quad column
-    auto bar = [] { named_sync(1, 32 * TK_WARPS); };
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::CREG));
+    constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
+    constexpr int KS = DT / 16, NT = 32 * C::WARPS;
+    const int grp = warp >> 2, wk = (warp & 3) * 16;   // units this warp's group takes, first key of the unit it takes
+    const int gr = lane >> 2, qc = lane & 3;           // fragment row (key or dimension) and column pair (query)
+    auto bar = [] { named_sync(1, NT); };
     uint8_t* qs = sm + C::q_off;
     float* merge = reinterpret_cast<float*>(sm + C::merge_off);
     float2* ml = reinterpret_cast<float2*>(sm + C::ml_off);
@@ -172,272 +237,253 @@ attn_token_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     int it = 0;
     bool ok = true;
     while (attn_next<C::ROWS, AT_KT>(a, run, &g)) {
-        // ---- q of the tile, in A-fragment order: {a0, a1, a2, a3} of k step ks, row tile mt at [mt][ks][lane]. The k
-        // order of a step of 16 is that of the codes' registers: slots 2c, 2c + 1, 2c + 8, 2c + 9 hold 4c .. 4c + 3.
-        {
-            const int nt = 32 * TK_WARPS, tid = threadIdx.x;
-            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-                // a power of two that brings the row's largest magnitude into [2^13, 2^14)
-                for (int r = tid >> 4; r < C::ROWS; r += nt >> 4) {
-                    float m = 0.f;
-                    if (r < g.rows) {
-                        const int t = (g.r0 + r) / a.G, hq = g.h * a.G + (g.r0 + r) - t * a.G;
-                        const T* q = reinterpret_cast<const T*>(a.q) + (g.q0 + t) * a.ldq + (long long)hq * a.dim;
-                        for (int d = 2 * (tid & 15); d < a.dim; d += 32) {
-                            const uint32_t w = *reinterpret_cast<const uint32_t*>(q + d);
-                            m = fmaxf(m, fmaxf(fabsf(__uint_as_float(w << 16)), fabsf(__uint_as_float(w & 0xffff0000u))));
-                        }
-                    }
+        // ---- q: registers of every warp, or shared memory ----
+        uint2 qr[C::QREGS ? KS : 1];
+        float qf[NQ][2];   // scale * log2(e) over the factor of this thread's queries 8 nq + 2 qc + {0, 1}
+        if constexpr (C::QREGS) {
+            const float f = tk_load_q<DT, T>(a, g, 0, lane, qr);
+            qf[0][0] = __fdiv_rn(a.scale_log2, __shfl_sync(0xffffffffu, f, 8 * qc));
+            qf[0][1] = __fdiv_rn(a.scale_log2, __shfl_sync(0xffffffffu, f, 8 * qc + 4));
+        } else {
+            if (warp < NQ) {
+                uint2 w[KS];
+                const float f = tk_load_q<DT, T>(a, g, warp, lane, w);
 #pragma unroll
-                    for (int o = 8; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                    if ((tid & 15) == 0) {
-                        const int e = (int)(__float_as_uint(m) >> 23) - 127;             // floor(log2 m); 0 or tiny: -127
-                        rowf[r] = m == 0.f ? 1.f : exp2f((float)min(126, max(-126, 13 - e)));
-                    }
-                }
-                bar();
-            }
-            constexpr int KS = DT / 16;
-            for (int i = tid; i < MT * KS * 32; i += nt) {
-                const int l = i & 31, ks = (i >> 5) % KS, mt = (i >> 5) / KS, d = 16 * ks + 4 * (l & 3);
-                uint2 w[2];
-#pragma unroll
-                for (int hl = 0; hl < 2; ++hl) {
-                    const int r = 16 * mt + (l >> 2) + 8 * hl;
-                    w[hl] = make_uint2(0u, 0u);
-                    if (r < g.rows && d < a.dim) {
-                        const int t = (g.r0 + r) / a.G, hq = g.h * a.G + (g.r0 + r) - t * a.G;
-                        const T* q = reinterpret_cast<const T*>(a.q) + (g.q0 + t) * a.ldq + (long long)hq * a.dim + d;
-                        w[hl] = *reinterpret_cast<const uint2*>(q);
-                        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-                            const float f = rowf[r];
-                            w[hl].x = pack_f16(__uint_as_float(w[hl].x << 16) * f, __uint_as_float(w[hl].x & 0xffff0000u) * f);
-                            w[hl].y = pack_f16(__uint_as_float(w[hl].y << 16) * f, __uint_as_float(w[hl].y & 0xffff0000u) * f);
-                        }
-                    }
-                }
-                *reinterpret_cast<uint4*>(qs + 16 * i) = make_uint4(w[0].x, w[1].x, w[0].y, w[1].y);
+                for (int ks = 0; ks < KS; ++ks) reinterpret_cast<uint2*>(qs)[(warp * KS + ks) * 32 + lane] = w[ks];
+                if (qc == 0) rowf[8 * warp + gr] = f;
             }
             bar();
+#pragma unroll
+            for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    qf[nq][e] = bf ? __fdiv_rn(a.scale_log2, rowf[8 * nq + 2 * qc + e]) : a.scale_log2;
         }
-        // rows of this thread: 16 mt + gr + 8 hl; keys [klo, khi) that each sees
-        int klo[MT][2], khi[MT][2];
-        float qf[MT][2];   // scale * log2(e), and the inverse of the row's factor
+        // keys [klo, khi) that this thread's queries see
+        int klo[NQ][2], khi[NQ][2];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
-            for (int hl = 0; hl < 2; ++hl) {
-                const int r = 16 * mt + gr + 8 * hl, rr = min(r, g.rows - 1);
+            for (int e = 0; e < 2; ++e) {
+                const int r = 8 * nq + 2 * qc + e, rr = min(r, g.rows - 1);
                 const int p = g.pos0 + (g.r0 + rr) / a.G;
-                khi[mt][hl] = r < g.rows ? p + 1 : 0;
-                klo[mt][hl] = a.window > 0 ? p - a.window + 1 : 0;
-                qf[mt][hl] = a.scale_log2;
-                if constexpr (std::is_same<T, __nv_bfloat16>::value) qf[mt][hl] = __fdiv_rn(a.scale_log2, rowf[rr]);
+                khi[nq][e] = r < g.rows ? p + 1 : 0;
+                klo[nq][e] = a.window > 0 ? p - a.window + 1 : 0;
             }
-        // keys that every row of the tile sees: no mask needed
+        // keys that every row of the tile sees: no mask needed (rows past the tile's compute what is not written)
         const int all_hi = g.pos0 + g.r0 / a.G + 1;
         const int all_lo = a.window > 0 ? g.pos0 + (g.r0 + g.rows - 1) / a.G - a.window + 1 : 0;
 
-        float o[MT][DT / 8][4], m[MT][2], l[MT][2], cref = 0.f;   // o of 16 columns j: even columns [2j], odd [2j + 1]
+        float o[NQ][KS][4];   // O^T: dimension 16 j + 2 gr (and + 1: elements 2, 3), queries 2 qc, 2 qc + 1
+        float M[NQ][2], l[NQ][2], V = 7.888609e-31f, vinv = 1.2676506e30f;   // 2^-100
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
+        for (int nq = 0; nq < NQ; ++nq) {
 #pragma unroll
-            for (int j = 0; j < DT / 8; ++j)
+            for (int j = 0; j < KS; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[mt][j][e] = 0.f;
-            m[mt][0] = m[mt][1] = -INFINITY;
-            l[mt][0] = l[mt][1] = 0.f;
+                for (int e = 0; e < 4; ++e) o[nq][j][e] = 0.f;
+            M[nq][0] = M[nq][1] = -INFINITY;
+            l[nq][0] = l[nq][1] = 0.f;
         }
-        for (int t = g.t0; t < g.t1; ++t, ++it) {
-            if ((it & 1) != grp) continue;
-            const int st = it % C::NS;
-            if (ok) ok = __all_sync(0xffffffffu, wait_parity(&full[st], (it / C::NS) & 1));
+        const int n = max(0, g.t1 - g.t0);
+        // this group's units: it + i with (it + i) % GROUPS == grp
+        for (int i = (grp - it) & (C::GROUPS - 1); i < n; i += C::GROUPS) {
+            const int u = it + i, st = u % C::NS;
+            if (ok) ok = __all_sync(0xffffffffu, wait_parity(&full[st], (u / C::NS) & 1));
             if (!ok) continue;   // the wait gave up (status bit): the walk goes on so that every arrival is made
             const uint32_t kt = smem_u32(sm + st * C::STAGE), vt = kt + C::TILE;
-            const int key0 = t * AT_KT + wk;
-            const int piece = a.page_log2 >= 6 ? 0 : wk >> a.page_log2;
+            const int key0 = (g.t0 + i) * AT_KT + wk;
             if (key0 < g.len) {
-                const float ks = scales[st * 8 + 2 * piece], vs = scales[st * 8 + 2 * piece + 1];
-                float s[MT][2][4];
+                const int piece = a.page_log2 >= 6 ? 0 : wk >> a.page_log2;
+                const float2 sc = *reinterpret_cast<const float2*>(scales + st * 8 + 2 * piece);
+                float s[NQ][4];
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+                for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
-                    for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) s[mt][nt][e] = 0.f;
+                    for (int e = 0; e < 4; ++e) s[nq][e] = 0.f;
 #pragma unroll
                 for (int c4 = 0; c4 < DT / 64; ++c4) {
                     uint32_t r0[4], r1[4];
                     ldsm_x4(r0, code_addr<DT>(kt, wk + (lane & 7), 4 * c4 + (lane >> 3)));
                     ldsm_x4(r1, code_addr<DT>(kt, wk + 8 + (lane & 7), 4 * c4 + (lane >> 3)));
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t b0 = codes_f16(r0[i], 0x4140u), b1 = codes_f16(r0[i], 0x4342u);
-                        const uint32_t b2 = codes_f16(r1[i], 0x4140u), b3 = codes_f16(r1[i], 0x4342u);
+                    for (int h = 0; h < 4; ++h) {
+                        const int ks = 4 * c4 + h;
+                        const uint32_t a0 = codes_f16(r0[h], 0x4140u), a1 = codes_f16(r1[h], 0x4140u);
+                        const uint32_t a2 = codes_f16(r0[h], 0x4342u), a3 = codes_f16(r1[h], 0x4342u);
 #pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) {
-                            const uint4 qa = lds128(smem_u32(qs) + 16 * ((mt * (DT / 16) + 4 * c4 + i) * 32 + lane));
-                            mma_16816(s[mt][0], qa.x, qa.y, qa.z, qa.w, b0, b1);
-                            mma_16816(s[mt][1], qa.x, qa.y, qa.z, qa.w, b2, b3);
+                        for (int nq = 0; nq < NQ; ++nq) {
+                            uint2 b;
+                            if constexpr (C::QREGS) b = qr[ks];
+                            else b = lds64(smem_u32(qs) + 8 * ((nq * KS + ks) * 32 + lane));
+                            mma_f16(s[nq], a0, a1, a2, a3, b.x, b.y);
                         }
                     }
                 }
-                // ---- scores in the log2 domain, masks, running maximum ----
+                if (sc.y > V) {   // the reference of V's scales follows (the warp together)
+                    const float f = V * __fdiv_rn(1.f, sc.y);
+                    V = sc.y;
+                    vinv = __fdiv_rn(1.f, V);
+#pragma unroll
+                    for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+                        for (int j = 0; j < KS; ++j)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[nq][j][e] *= f;
+                }
+                const float ratio = fmaxf(sc.y * vinv, 9.313226e-10f);   // vs / V, at least 2^-30
+                const float lv = __log2f(ratio), iv = __fdividef(1.f, ratio);
                 const bool masked = key0 + 16 > all_hi || key0 < all_lo;
-                bool grow = false;
-                float top[MT][2];
+                uint32_t pk[NQ][2];   // p' of keys gr and gr + 8
+                float add[NQ][2];
+                auto weigh = [&] {
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int hl = 0; hl < 2; ++hl) {
-                        const float f = qf[mt][hl] * ks;
-                        float x = -INFINITY;
-#pragma unroll
-                        for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                float v = s[mt][nt][2 * hl + e] * f;
-                                if (masked) {
-                                    const int j = key0 + 8 * nt + 2 * qc + e;
-                                    if (j < klo[mt][hl] || j >= khi[mt][hl]) v = -INFINITY;
-                                }
-                                s[mt][nt][2 * hl + e] = v;
-                                x = fmaxf(x, v);
-                            }
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-                        top[mt][hl] = x;
-                        grow |= x > m[mt][hl] + TK_LAZY || (x > -INFINITY && m[mt][hl] == -INFINITY);
-                    }
-                const bool cgrow = vs > cref;
-                if (__any_sync(0xffffffffu, grow) || cgrow) {
-                    const float cf = cgrow ? (cref > 0.f ? __fdiv_rn(cref, vs) : 0.f) : 1.f;
-                    if (cgrow) cref = vs;
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                        for (int hl = 0; hl < 2; ++hl) {
-                            const float mn = fmaxf(m[mt][hl], top[mt][hl]);
-                            const float al = m[mt][hl] == -INFINITY ? 0.f : ex2(m[mt][hl] - mn);
-                            m[mt][hl] = mn;
-                            l[mt][hl] *= al;
-                            const float af = al * cf;
-#pragma unroll
-                            for (int j = 0; j < DT / 8; ++j) {
-                                o[mt][j][2 * hl] *= af;
-                                o[mt][j][2 * hl + 1] *= af;
-                            }
-                        }
-                }
-                const float vf = cref > 0.f ? __fdiv_rn(vs, cref) : 0.f;   // <= 1
-                uint32_t pa[MT][4];
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int hl = 0; hl < 2; ++hl) {
-                        const float mr = m[mt][hl] == -INFINITY ? 0.f : m[mt][hl] - TK_P_BIAS;
+                    for (int nq = 0; nq < NQ; ++nq) {
                         float p[4];
 #pragma unroll
-                        for (int nt = 0; nt < 2; ++nt)
+                        for (int e = 0; e < 2; ++e) {
+                            const float kf = qf[nq][e] * sc.x, cg = lv - (M[nq][e] == -INFINITY ? 0.f : M[nq][e] - TK_P_BIAS);
 #pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                p[2 * nt + e] = ex2(s[mt][nt][2 * hl + e] - mr);
-                                l[mt][hl] += p[2 * nt + e];
+                            for (int h = 0; h < 2; ++h) {
+                                float x = fmaf(s[nq][2 * h + e], kf, cg);
+                                if (masked) {
+                                    const int j = key0 + gr + 8 * h;
+                                    if (j < klo[nq][e] || j >= khi[nq][e]) x = -INFINITY;
+                                }
+                                p[2 * h + e] = ex2(x);
                             }
-                        pa[mt][hl] = pack_f16(p[0] * vf, p[1] * vf);
-                        pa[mt][2 + hl] = pack_f16(p[2] * vf, p[3] * vf);
+                            add[nq][e] = p[e] + p[2 + e];
+                        }
+                        pk[nq][0] = pack_f16(p[0], p[1]);
+                        pk[nq][1] = pack_f16(p[2], p[3]);
                     }
-                // ---- o += p c' ----
+                };
+                weigh();
+                bool again = false;   // first keys of a row, or a p' past 2^12 (fp16 0x6c00; NaN, 0x7fff, too)
+#pragma unroll
+                for (int nq = 0; nq < NQ; ++nq) {
+                    const uint32_t top = h2_max(pk[nq][0], pk[nq][1]);
+                    again |= (top & 0xffffu) > 0x6c00u || (top >> 16) > 0x6c00u;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        again |= M[nq][e] == -INFINITY && klo[nq][e] < key0 + 16 && khi[nq][e] > key0;
+                }
+                if (__any_sync(0xffffffffu, again)) {
+#pragma unroll
+                    for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            float x = -INFINITY;
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const int j = key0 + gr + 8 * h;
+                                if (!masked || (j >= klo[nq][e] && j < khi[nq][e]))
+                                    x = fmaxf(x, fmaf(s[nq][2 * h + e], qf[nq][e] * sc.x, lv));
+                            }
+#pragma unroll
+                            for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+                            const float mn = fmaxf(M[nq][e], x), al = M[nq][e] == -INFINITY ? 0.f : ex2(M[nq][e] - mn);
+                            M[nq][e] = mn;
+                            l[nq][e] *= al;
+#pragma unroll
+                            for (int j = 0; j < KS; ++j) {
+                                o[nq][j][e] *= al;
+                                o[nq][j][2 + e] *= al;
+                            }
+                        }
+                    weigh();
+                }
+                uint32_t b[NQ][2];   // p'^T: keys as k, queries as columns
+#pragma unroll
+                for (int nq = 0; nq < NQ; ++nq) {
+                    l[nq][0] = fmaf(add[nq][0], iv, l[nq][0]);
+                    l[nq][1] = fmaf(add[nq][1], iv, l[nq][1]);
+                    b[nq][0] = movm(pk[nq][0]);
+                    b[nq][1] = movm(pk[nq][1]);
+                }
 #pragma unroll
                 for (int j2 = 0; j2 < DT / 32; ++j2) {
                     uint32_t r[4];
                     ldsm_x4_t(r, code_addr<DT>(vt, wk + 8 * ((lane >> 3) & 1) + (lane & 7), 2 * j2 + (lane >> 4)));
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const uint32_t e0 = codes_f16(r[2 * h], 0x4240u), e1 = codes_f16(r[2 * h + 1], 0x4240u);
-                        const uint32_t d0 = codes_f16(r[2 * h], 0x4341u), d1 = codes_f16(r[2 * h + 1], 0x4341u);
+                        const uint32_t a0 = codes_f16(r[2 * h], 0x4240u), a1 = codes_f16(r[2 * h], 0x4341u);
+                        const uint32_t a2 = codes_f16(r[2 * h + 1], 0x4240u), a3 = codes_f16(r[2 * h + 1], 0x4341u);
 #pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) {
-                            mma_16816(o[mt][2 * (2 * j2 + h)], pa[mt][0], pa[mt][1], pa[mt][2], pa[mt][3], e0, e1);
-                            mma_16816(o[mt][2 * (2 * j2 + h) + 1], pa[mt][0], pa[mt][1], pa[mt][2], pa[mt][3], d0, d1);
-                        }
+                        for (int nq = 0; nq < NQ; ++nq) mma_f16(o[nq][2 * j2 + h], a0, a1, a2, a3, b[nq][0], b[nq][1]);
                     }
                 }
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty[st]);
         }
-        // ---- join the warps: o of row r = sum_w o_w c_w 2^(m_w - M), l likewise ----
+        it += n;
+        // ---- join the warps: O of a row = sum_w V_w O_w 2^(M_w - M), l likewise ----
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
-            for (int hl = 0; hl < 2; ++hl) {
-                l[mt][hl] += __shfl_xor_sync(0xffffffffu, l[mt][hl], 1);
-                l[mt][hl] += __shfl_xor_sync(0xffffffffu, l[mt][hl], 2);
-                if (qc == 0) ml[warp * C::ROWS + 16 * mt + gr + 8 * hl] = make_float2(m[mt][hl], l[mt][hl]);
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) l[nq][e] += __shfl_xor_sync(0xffffffffu, l[nq][e], d);
+                if (gr == 0) ml[warp * C::ROWS + 8 * nq + 2 * qc + e] = make_float2(M[nq][e], l[nq][e]);
             }
         bar();
         const bool direct = g.whole;
         constexpr int PITCH = DT + 2;
         float* part = a.part + attn_slot(run, g, blockIdx.x) * C::ROWS * PITCH;
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            float mm[2], lsum[2], fac[2];
+        for (int nq = 0; nq < NQ; ++nq) {
+            float fac[2];
 #pragma unroll
-            for (int hl = 0; hl < 2; ++hl) {
-                const int r = 16 * mt + gr + 8 * hl;
-                mm[hl] = -INFINITY;
+            for (int e = 0; e < 2; ++e) {
+                const int r = 8 * nq + 2 * qc + e;
+                float mm = -INFINITY, lsum = 0.f;
 #pragma unroll
-                for (int w = 0; w < TK_WARPS; ++w) mm[hl] = fmaxf(mm[hl], ml[w * C::ROWS + r].x);
-                lsum[hl] = 0.f;
+                for (int w = 0; w < C::WARPS; ++w) mm = fmaxf(mm, ml[w * C::ROWS + r].x);
 #pragma unroll
-                for (int w = 0; w < TK_WARPS; ++w) {
+                for (int w = 0; w < C::WARPS; ++w) {
                     const float2 v = ml[w * C::ROWS + r];
-                    if (v.x > -INFINITY) lsum[hl] = fmaf(v.y, ex2(v.x - mm[hl]), lsum[hl]);
+                    if (v.x > -INFINITY) lsum = fmaf(v.y, ex2(v.x - mm), lsum);
                 }
-                fac[hl] = m[mt][hl] > -INFINITY ? ex2(m[mt][hl] - mm[hl]) * cref : 0.f;
-                if (direct) fac[hl] = lsum[hl] == 0.f ? 0.f : __fdiv_rn(fac[hl], lsum[hl]);
-                if (!direct && warp == 0 && qc == 0 && r < g.rows)
-                    *reinterpret_cast<float2*>(part + C::ROWS * DT + 2 * r) = make_float2(mm[hl], lsum[hl]);
+                fac[e] = M[nq][e] > -INFINITY ? ex2(M[nq][e] - mm) * V : 0.f;
+                if (direct) fac[e] = lsum == 0.f ? 0.f : __fdiv_rn(fac[e], lsum);
+                if (!direct && warp == 0 && gr == 0 && r < g.rows)
+                    *reinterpret_cast<float2*>(part + C::ROWS * DT + 2 * r) = make_float2(mm, lsum);
             }
 #pragma unroll
-            for (int c = 0; c < DT / 32; ++c) {
-                if (32 * c >= a.dim) break;
-                // 32 columns: two groups of 16, of which this thread holds 4 qc .. 4 qc + 3
+            for (int c = 0; c < DT / 64; ++c) {
+                if (64 * c >= a.dim) break;
+                // 64 columns, [warp][query][column]
 #pragma unroll
-                for (int jj = 0; jj < 2; ++jj)
+                for (int jj = 0; jj < 4; ++jj)
 #pragma unroll
-                    for (int hl = 0; hl < 2; ++hl) {
-                        const float* e = o[mt][2 * (2 * c + jj)];
-                        const float* d = o[mt][2 * (2 * c + jj) + 1];
-                        float* x = merge + (warp * 16 + gr + 8 * hl) * 32 + 16 * jj + 4 * qc;
-                        *reinterpret_cast<float4*>(x) = make_float4(e[2 * hl] * fac[hl], d[2 * hl] * fac[hl],
-                                                                    e[2 * hl + 1] * fac[hl], d[2 * hl + 1] * fac[hl]);
-                    }
+                    for (int e = 0; e < 2; ++e)
+                        *reinterpret_cast<float2*>(merge + (warp * 8 + 2 * qc + e) * 64 + 16 * jj + 2 * gr) =
+                            make_float2(o[nq][4 * c + jj][e] * fac[e], o[nq][4 * c + jj][2 + e] * fac[e]);
                 bar();
-                {
-                    const int r16 = threadIdx.x >> 4, d = 2 * (threadIdx.x & 15), r = 16 * mt + r16;
+                // two columns of a row per thread of the first 256
+                if (threadIdx.x < 256) {
+                    const int r8 = threadIdx.x >> 5, d = 2 * (threadIdx.x & 31), r = 8 * nq + r8;
                     float2 v = make_float2(0.f, 0.f);
 #pragma unroll
-                    for (int w = 0; w < TK_WARPS; ++w) {
-                        const float2 x = *reinterpret_cast<const float2*>(merge + (w * 16 + r16) * 32 + d);
+                    for (int w = 0; w < C::WARPS; ++w) {
+                        const float2 x = *reinterpret_cast<const float2*>(merge + (w * 8 + r8) * 64 + d);
                         v.x += x.x;
                         v.y += x.y;
                     }
-                    if (r < g.rows && 32 * c + d < a.dim) {
+                    if (r < g.rows && 64 * c + d < a.dim) {
                         if (direct) {
-                            T* out = attn_out<T>(a, g, r) + 32 * c + d;
-                            *reinterpret_cast<uint32_t*>(out) =
-                                std::is_same<T, __half>::value ? pack_f16(v.x, v.y) : pack_bf16(v.x, v.y);
+                            T* out = attn_out<T>(a, g, r) + 64 * c + d;
+                            *reinterpret_cast<uint32_t*>(out) = bf ? pack_bf16(v.x, v.y) : pack_f16(v.x, v.y);
                         } else {
-                            *reinterpret_cast<float2*>(part + ((8 * c + (d >> 2)) * C::ROWS + r) * 4 + (d & 3)) = v;
+                            *reinterpret_cast<float2*>(part + ((16 * c + (d >> 2)) * C::ROWS + r) * 4 + (d & 3)) = v;
                         }
                     }
                 }
                 bar();
             }
         }
-        if (!direct) attn_join<DT, C::ROWS, T>(a, run, g, threadIdx.x, 32 * TK_WARPS, join_sh, bar);
+        if (!direct) attn_join<DT, C::ROWS, T>(a, run, g, threadIdx.x, NT, join_sh, bar);
     }
 }
 
