@@ -18,9 +18,16 @@ static size_t attn_part_floats(int dt) {
     return (size_t)(dt == 256 ? 128 : 256) * (dt + 2);   // the prompt kernel's tile is the larger one
 }
 
+// Whether the kernels' 32-bit unit counts hold the call: an upper bound of its items times their units.
+static bool units_fit(const vkb_kv_cache_t* c, const AttnArgs& a, int rows, int keys, int own) {
+    const double items = (double)a.heads * ((double)a.T * a.G / rows + a.B);
+    return items * ((double)a.table_ld * c->page / keys + 1 + own) <= 2147483647.0;
+}
+
 template <int DT, int NQ, typename T>
 static int launch_token(const vkb_kv_cache_t* c, const AttnArgs& a, int dev, cudaStream_t st) {
     using C = TkCfg<DT, NQ>;
+    if (!units_fit(c, a, C::ROWS, AT_KT, TK_OV)) return VKB_EUNSUPPORTED;
     auto kern = attn_token_kernel<DT, NQ, T>;
     static std::once_flag once[kMaxDevices];
     static cudaError_t err[kMaxDevices];
@@ -44,6 +51,7 @@ static int launch_token(const vkb_kv_cache_t* c, const AttnArgs& a, int dev, cud
 template <int DT, typename T>
 static int launch_prompt(const vkb_kv_cache_t* c, const AttnArgs& a, int dev, cudaStream_t st) {
     using C = PrCfg<DT>;
+    if (!units_fit(c, a, C::ROWS, PR_KT, PR_OV)) return VKB_EUNSUPPORTED;
     auto kern = attn_prompt_kernel<DT, T>;
     static std::once_flag once[kMaxDevices];
     static cudaError_t err[kMaxDevices];

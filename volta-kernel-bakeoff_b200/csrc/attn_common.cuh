@@ -4,7 +4,9 @@
 // A work item is one sequence, one kv head and one tile of ROWS query rows; row r of a sequence is query token r / G,
 // head h G + r % G (G = q heads per kv head), so that the heads sharing a kv head read its codes once. An item's units
 // are its tiles of KT keys, from the first key that any of its rows sees to the last (an item that sees none has one
-// empty unit, which writes its zeros). The units of all items, in order, are dealt out to the thread blocks in equal
+// empty unit, which writes its zeros), and OV more in front of them, which stand for what an item costs beside its keys
+// (q, the joining of the warps, the output; measured at 16 for both kernels: a batch of 64 sequences of 1 to 8192 tokens 168 us
+// without, 111 us with them, ragged prompts through a window 906 and 483 us). The units of all items, in order, are dealt out to the thread blocks in equal
 // contiguous runs, worked out on the device from the lengths there: ragged batches balance, nothing is read back to
 // the host, and a captured graph stays right as sequences grow. An item cut by a run's border is a "part" in each
 // block: its unnormalised sums go to the workspace, and the block that arrives last joins the parts in block order
@@ -56,23 +58,23 @@ template <int KT> __device__ __forceinline__ void attn_tiles(const AttnArgs& a, 
     *t1 = last >= 0 ? (last + KT) / KT : 0;
     if (*t1 < *t0) *t1 = *t0;
 }
-template <int KT> __device__ __forceinline__ int attn_units(const AttnArgs& a, const AttnSeq& s, int r0, int r1) {
+template <int KT, int OV> __device__ __forceinline__ int attn_units(const AttnArgs& a, const AttnSeq& s, int r0, int r1) {
     int t0, t1;
     attn_tiles<KT>(a, s, r0, r1, &t0, &t1);
-    return max(1, t1 - t0);
+    return max(1, t1 - t0) + OV;
 }
 // Units of one head of a sequence.
-template <int ROWS, int KT> __device__ __forceinline__ long long attn_head_units(const AttnArgs& a, const AttnSeq& s) {
+template <int ROWS, int KT, int OV> __device__ __forceinline__ unsigned attn_head_units(const AttnArgs& a, const AttnSeq& s) {
     const int rows = s.n * a.G;
-    long long u = 0;
-    for (int r = 0; r < rows; r += ROWS) u += attn_units<KT>(a, s, r, min(rows, r + ROWS));
+    unsigned u = 0;
+    for (int r = 0; r < rows; r += ROWS) u += (unsigned) attn_units<KT, OV>(a, s, r, min(rows, r + ROWS));
     return u;
 }
 
-// A run of units: where it starts, and the walk over its segments.
+// A run of units: where it starts, and the walk over its segments. (The host refuses calls that could have 2^31 units.)
 struct AttnRun {
-    long long u, u1, total;   // next unit, end of the run, units of the call
-    int nb;                   // blocks with a run
+    unsigned u, u1;           // next unit, end of the run
+    unsigned per, rem;        // block c's run: per units from c per + min(c, rem) on, one more where c < rem
     int b, h, r0, off;        // next item and the units of it that belong to earlier blocks
 };
 struct AttnSeg {
@@ -80,68 +82,69 @@ struct AttnSeg {
     int pos0, q0;             // position of the sequence's first query token, its row in q and out
     int t0, t1;               // key tiles of this segment
     int len;
-    long long iu0, iu1;       // the whole item's units
+    int c0, c1;               // blocks that hold the item (c0 == c1: this one, whole)
     bool whole;
 };
 
-// First unit of block c's run.
-__device__ __forceinline__ long long attn_start(long long total, int nb, int c) { return total * c / nb; }
+__device__ __forceinline__ unsigned attn_start(const AttnRun& r, int c) { return c * r.per + min((unsigned)c, r.rem); }
 // The block whose run holds unit x.
-__device__ __forceinline__ int attn_owner(long long total, int nb, long long x) {
-    return (int)(((x + 1) * nb - 1) / total);
+__device__ __forceinline__ int attn_owner(const AttnRun& r, unsigned x) {
+    const unsigned big = r.rem * (r.per + 1);
+    return (int)(x < big ? x / (r.per + 1) : r.rem + (x - big) / r.per);
 }
 
-// All threads of the block: this block's run. sh: 2 + NT / 32 words of 8 bytes of shared memory.
-template <int ROWS, int KT, int NT> __device__ __forceinline__ AttnRun attn_run(const AttnArgs& a, long long* sh) {
+// All threads of the block: this block's run. sh: 2 + NT / 32 words of shared memory.
+template <int ROWS, int KT, int OV, int NT> __device__ __forceinline__ AttnRun attn_run(const AttnArgs& a, unsigned* sh) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int NW = NT / 32;
     AttnRun r;
-    long long total = 0, mine0 = 0;
+    unsigned total = 0, mine0 = 0;
     for (int b = tid; b < a.B; b += NT) {
         const AttnSeq s = attn_seq(a, b);
-        const long long u = a.heads * attn_head_units<ROWS, KT>(a, s);
+        const unsigned u = a.heads * attn_head_units<ROWS, KT, OV>(a, s);
         if (b == tid) mine0 = u;
         total += u;
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    total = __reduce_add_sync(0xffffffffu, total);
     if (lane == 0) sh[warp] = total;
     __syncthreads();
     total = 0;
 #pragma unroll
     for (int w = 0; w < NW; ++w) total += sh[w];
     __syncthreads();
-    r.total = total;
-    r.nb = (int)min((long long)gridDim.x, total);
-    r.u = r.u1 = 0;
+    const unsigned nb = min(gridDim.x, total);
+    r.u = r.u1 = r.rem = 0;
+    r.per = 1;
     r.b = r.h = r.r0 = r.off = 0;
-    if ((int)blockIdx.x >= r.nb) return r;
-    r.u = attn_start(total, r.nb, blockIdx.x);
-    r.u1 = attn_start(total, r.nb, blockIdx.x + 1);
+    if (blockIdx.x >= nb) return r;
+    r.per = total / nb;
+    r.rem = total - r.per * nb;
+    r.u = attn_start(r, blockIdx.x);
+    r.u1 = attn_start(r, blockIdx.x + 1);
     // the sequence that holds unit r.u: a scan, NT sequences at a time
-    long long left = r.u;
+    unsigned left = r.u;
     for (int base = 0; base < a.B; base += NT) {
         const int b = base + tid;
-        long long u = mine0;
-        if (base > 0) u = b < a.B ? a.heads * attn_head_units<ROWS, KT>(a, attn_seq(a, b)) : 0;
-        long long inc = u;
+        unsigned u = mine0;
+        if (base > 0) u = b < a.B ? a.heads * attn_head_units<ROWS, KT, OV>(a, attn_seq(a, b)) : 0;
+        unsigned inc = u;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+            const unsigned v = __shfl_up_sync(0xffffffffu, inc, o);
             if (lane >= o) inc += v;
         }
         if (lane == 31) sh[warp] = inc;
         __syncthreads();
-        long long before = 0, all = 0;
+        unsigned before = 0, all = 0;
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
             before += w < warp ? sh[w] : 0;
             all += sh[w];
         }
-        const long long at = left - (before + inc - u);
-        if (at >= 0 && at < u) {
-            sh[NW] = b;
-            sh[NW + 1] = at;
+        before += inc - u;
+        if (left >= before && left - before < u) {
+            sh[NW] = (unsigned)b;
+            sh[NW + 1] = left - before;
         }
         __syncthreads();
         if (left < all) break;
@@ -149,13 +152,13 @@ template <int ROWS, int KT, int NT> __device__ __forceinline__ AttnRun attn_run(
     }
     r.b = (int)sh[NW];
     const AttnSeq s = attn_seq(a, r.b);
-    const long long per = attn_head_units<ROWS, KT>(a, s);
-    long long at = sh[NW + 1];
+    const unsigned per = attn_head_units<ROWS, KT, OV>(a, s);
+    unsigned at = sh[NW + 1];
     r.h = (int)(at / per);
     at -= r.h * per;
     const int rows = s.n * a.G;
     for (;; r.r0 += ROWS) {
-        const int u = attn_units<KT>(a, s, r.r0, min(rows, r.r0 + ROWS));
+        const unsigned u = (unsigned)attn_units<KT, OV>(a, s, r.r0, min(rows, r.r0 + ROWS));
         if (at < u) break;
         at -= u;
     }
@@ -164,47 +167,52 @@ template <int ROWS, int KT, int NT> __device__ __forceinline__ AttnRun attn_run(
 }
 
 // The run's next segment; false at its end.
-template <int ROWS, int KT> __device__ __forceinline__ bool attn_next(const AttnArgs& a, AttnRun& r, AttnSeg* g) {
-    if (r.u >= r.u1) return false;
-    AttnSeq s = attn_seq(a, r.b);
-    while (s.n == 0) {   // sequences without query tokens have no unit
-        if (r.b + 1 >= a.B) return false;
-        s = attn_seq(a, ++r.b);
-    }
-    const int rows = s.n * a.G;
-    g->b = r.b;
-    g->h = r.h;
-    g->r0 = r.r0;
-    g->rows = min(ROWS, rows - r.r0);
-    g->pos0 = s.len - s.n;
-    g->q0 = s.q0;
-    g->len = s.len;
-    int t0, t1;
-    attn_tiles<KT>(a, s, r.r0, r.r0 + g->rows, &t0, &t1);
-    const int units = max(1, t1 - t0);
-    const int take = (int)min((long long)(units - r.off), r.u1 - r.u);
-    g->iu0 = r.u - r.off;
-    g->iu1 = g->iu0 + units;
-    g->whole = take == units;
-    g->t0 = t0 + r.off;
-    g->t1 = min(t1, g->t0 + take);
-    r.u += take;
-    r.off = 0;
-    r.r0 += ROWS;
-    if (r.r0 >= rows) {
-        r.r0 = 0;
-        if (++r.h == a.heads) {
-            r.h = 0;
-            ++r.b;
+template <int ROWS, int KT, int OV> __device__ __forceinline__ bool attn_next(const AttnArgs& a, AttnRun& r, AttnSeg* g) {
+    for (;;) {
+        if (r.u >= r.u1) return false;
+        AttnSeq s = attn_seq(a, r.b);
+        while (s.n == 0) {   // sequences without query tokens have no unit
+            if (r.b + 1 >= a.B) return false;
+            s = attn_seq(a, ++r.b);
         }
+        const int rows = s.n * a.G;
+        g->b = r.b;
+        g->h = r.h;
+        g->r0 = r.r0;
+        g->rows = min(ROWS, rows - r.r0);
+        g->pos0 = s.len - s.n;
+        g->q0 = s.q0;
+        g->len = s.len;
+        int t0, t1;
+        attn_tiles<KT>(a, s, r.r0, r.r0 + g->rows, &t0, &t1);
+        const int units = max(1, t1 - t0) + OV;
+        const int off = r.off, take = (int)min((unsigned)(units - off), r.u1 - r.u);
+        const unsigned first = r.u - off;   // the item's first unit
+        r.u += take;
+        r.off = 0;
+        r.r0 += ROWS;
+        if (r.r0 >= rows) {
+            r.r0 = 0;
+            if (++r.h == a.heads) {
+                r.h = 0;
+                ++r.b;
+            }
+        }
+        if (off + take <= OV) continue;   // nothing but the units in front: the next block has the item's first keys
+        g->whole = off <= OV && off + take == units;
+        g->c0 = g->c1 = blockIdx.x;
+        if (!g->whole) {
+            g->c0 = attn_owner(r, first + OV);
+            g->c1 = attn_owner(r, first + units - 1);
+        }
+        g->t0 = t0 + max(0, off - OV);
+        g->t1 = min(t1, t0 + off + take - OV);
+        return true;
     }
-    return true;
 }
 
-// Where a part of this block goes: slot 1 for the item that starts in the block, 0 for one that started earlier.
-__device__ __forceinline__ long long attn_slot(const AttnRun& r, const AttnSeg& g, int c) {
-    return 2ll * c + (attn_owner(r.total, r.nb, g.iu0) == c ? 1 : 0);
-}
+// Where a part of block c goes: slot 1 for the item that starts in the block, 0 for one that started earlier.
+__device__ __forceinline__ long long attn_slot(const AttnSeg& g, int c) { return 2ll * c + (g.c0 == c ? 1 : 0); }
 
 // Output row of row r of a segment.
 template <typename T> __device__ __forceinline__ T* attn_out(const AttnArgs& a, const AttnSeg& g, int r) {
@@ -216,42 +224,73 @@ template <typename T> __device__ __forceinline__ T* attn_out(const AttnArgs& a, 
 // the segment's item, and where this block is the last, join its parts and write the output. bar: a barrier among the n
 // threads. sh: a word of shared memory that they share.
 template <int DT, int ROWS, typename T, typename Bar>
-__device__ __forceinline__ void attn_join(const AttnArgs& a, const AttnRun& r, const AttnSeg& g, int tid, int n,
-                                          volatile int* sh, Bar bar) {
-    const int c0 = attn_owner(r.total, r.nb, g.iu0), c1 = attn_owner(r.total, r.nb, g.iu1 - 1), parts = c1 - c0 + 1;
+__device__ __forceinline__ void attn_join(const AttnArgs& a, const AttnSeg& g, int tid, int n, volatile int* sh, Bar bar) {
+    const int parts = g.c1 - g.c0 + 1;
     __threadfence();   // this thread's part, before the arrival
     bar();
     if (tid == 0) {
         __threadfence();
-        *sh = atomicInc(&a.cnt[c0], (unsigned)(parts - 1)) == (unsigned)(parts - 1);   // wraps to zero
+        *sh = atomicInc(&a.cnt[g.c0], (unsigned)(parts - 1)) == (unsigned)(parts - 1);   // wraps to zero
         __threadfence();
     }
     bar();
     if (!*sh) return;
-    constexpr int PITCH = DT + 2;
-    const float* base = a.part;
-    auto slot = [&](int c) { return base + (2ll * c + (c == c0 ? 1 : 0)) * ROWS * PITCH; };
-    // A thread takes four columns of a row; neighbouring threads neighbouring rows, as the parts lie.
-    const int work = g.rows * (a.dim >> 2);
-    for (int i = tid; i < work; i += n) {
-        const int d4 = i / g.rows, row = i - d4 * g.rows;
-        float m = -INFINITY;
-#pragma unroll 8
-        for (int c = c0; c <= c1; ++c) m = fmaxf(m, __ldcg(slot(c) + ROWS * DT + 2 * row));
-        if (m == -INFINITY) m = 0.f;   // no part saw a key
-        float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-        for (int c = c0; c <= c1; ++c) {
-            const float* p = slot(c);
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p + ROWS * DT + 2 * row));
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(p) + d4 * ROWS + row);
-            const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);
-            l = fmaf(w, ml.y, l);
-            o[0] = fmaf(w, v.x, o[0]);
-            o[1] = fmaf(w, v.y, o[1]);
-            o[2] = fmaf(w, v.z, o[2]);
-            o[3] = fmaf(w, v.w, o[3]);
+    constexpr int PITCH = DT + 2, BATCH = 8;
+    // A thread takes four columns of a row; neighbouring threads neighbouring rows, as the parts lie. Where there are
+    // threads for it, four lanes share an item's parts and add their sums up (in a fixed order).
+    const int work = g.rows * (a.dim >> 2), sp = parts > 4 && work * 4 <= n ? 4 : 1;
+    for (int i0 = 0; i0 < work * sp; i0 += n) {   // every lane takes every turn: the lanes that share an item shuffle
+        const int i = (i0 + tid) / sp, k = (i0 + tid) % sp;
+        const bool on = i < work;
+        const int d4 = on ? i / g.rows : 0, row = on ? i - d4 * g.rows : 0;
+        float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int c = k; c < parts; c += BATCH * sp) {
+            float2 ml[BATCH];
+            float4 v[BATCH];
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j) {
+                const int p = c + j * sp;
+                ml[j] = make_float2(-INFINITY, 0.f);
+                v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (p < parts) {
+                    const float* at = a.part + attn_slot(g, g.c0 + p) * ROWS * PITCH;
+                    ml[j] = __ldcg(reinterpret_cast<const float2*>(at + ROWS * DT + 2 * row));
+                    v[j] = __ldcg(reinterpret_cast<const float4*>(at) + d4 * ROWS + row);
+                }
+            }
+            float mn = m;
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j) mn = fmaxf(mn, ml[j].x);
+            const float mu = mn == -INFINITY ? 0.f : mn, f = exp2f(m - mu);   // nothing seen so far: 0
+            l *= f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] *= f;
+            m = mn;
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j) {
+                const float w = exp2f(ml[j].x - mu);
+                l = fmaf(w, ml[j].y, l);
+                o[0] = fmaf(w, v[j].x, o[0]);
+                o[1] = fmaf(w, v[j].y, o[1]);
+                o[2] = fmaf(w, v[j].z, o[2]);
+                o[3] = fmaf(w, v[j].w, o[3]);
+            }
         }
+        if (sp == 4) {
+            float mn = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 2));
+            const float f = exp2f(m - (mn == -INFINITY ? 0.f : mn));
+            l *= f;
+            l += __shfl_xor_sync(0xffffffffu, l, 1);
+            l += __shfl_xor_sync(0xffffffffu, l, 2);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                o[e] *= f;
+                o[e] += __shfl_xor_sync(0xffffffffu, o[e], 1);
+                o[e] += __shfl_xor_sync(0xffffffffu, o[e], 2);
+            }
+        }
+        if (!on || k != 0) continue;
         const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
         uint2 w;
         if constexpr (std::is_same<T, __half>::value)

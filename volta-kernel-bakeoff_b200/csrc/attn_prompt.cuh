@@ -28,6 +28,7 @@
 namespace vkb {
 
 constexpr int PR_KT = 64;                // keys per unit
+constexpr int PR_OV = 16;                // an item's own cost in units
 constexpr int PR_THREADS = 512;
 constexpr float PR_BIAS = 8.f;           // p' carries 2^8
 constexpr int PR_SCT = 16;               // tiles of scale tables: two batches of eight (a lane per group of 16 keys)
@@ -48,7 +49,7 @@ template <int DT> struct PrCfg {
     static constexpr int bar_off = row_off + ROWS * 4;
     static constexpr int NBAR = 1 + 4 * NS + 4 + 4 + 4 + 4;
     static constexpr int run_off = bar_off + NBAR * 8;
-    static constexpr int BYTES = run_off + 8 * (PR_THREADS / 32 + 2) + 32 + 1024;
+    static constexpr int BYTES = run_off + 4 * (PR_THREADS / 32 + 2) + 16 + 1024;
     static constexpr int o_col = 256;                             // O of row tile t at o_col + t DT; its S buffers at
                                                                   // 128 t and 128 t + 64
 };
@@ -187,7 +188,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
     uint64_t* o_full = p_full + 4;        // [2 t + tile parity] O of the row tile updated
     uint64_t* sc_full = o_full + 4;       // [2] eight tiles' scale tables written
     uint64_t* sc_empty = sc_full + 2;     // [2] and read (NT * 4 warps)
-    long long* run_sh = reinterpret_cast<long long*>(sm + C::run_off);
+    unsigned* run_sh = reinterpret_cast<unsigned*>(sm + C::run_off);
     volatile int* join_sh = reinterpret_cast<volatile int*>(run_sh + PR_THREADS / 32 + 2);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(run_sh + PR_THREADS / 32 + 2) + 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -215,7 +216,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
     if (warp == 0) tmem_alloc<1>(tmem_slot, 512);
     tc_fence_before();
     pdl_wait();
-    AttnRun run = attn_run<C::ROWS, PR_KT, PR_THREADS>(a, run_sh);   // its barriers publish the above
+    AttnRun run = attn_run<C::ROWS, PR_KT, PR_OV, PR_THREADS>(a, run_sh);   // its barriers publish the above
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     AttnSeg g;
@@ -252,7 +253,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
             }
             __syncwarp();
         };
-        while (ok && attn_next<C::ROWS, PR_KT>(a, run, &g)) {
+        while (ok && attn_next<C::ROWS, PR_KT, PR_OV>(a, run, &g)) {
             const int n = g.t1 - g.t0;
             if (n <= 0) continue;
             wait(q_full, qn++);
@@ -283,7 +284,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
         } else if (warp == 1) {
         // ===================== scale tables =====================
         int nb = 0;   // batches so far
-        while (ok && attn_next<C::ROWS, PR_KT>(a, run, &g)) {
+        while (ok && attn_next<C::ROWS, PR_KT, PR_OV>(a, run, &g)) {
             const int n = g.t1 - g.t0;
             float vs0 = 0.f, cmax = 0.f;   // reference and largest V scale of the segment
             int next = pr_page(a, g, g.t0, lane);
@@ -343,7 +344,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
             }
         };
         struct Tile { uint4 k[NB], v[NB]; };   // a tile's codes on their way to shared memory
-        while (ok && attn_next<C::ROWS, PR_KT>(a, run, &g)) {
+        while (ok && attn_next<C::ROWS, PR_KT, PR_OV>(a, run, &g)) {
             const int n = g.t1 - g.t0;
             // eight tiles' groups, a lane each: where their codes start, -1 where there are none
             long long base = -1;
@@ -410,7 +411,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
         const int nsm = 128 * NT, stid = threadIdx.x - 128;
         auto bar = [&] { named_sync(1, (uint32_t)nsm); };
         constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
-        while (attn_next<C::ROWS, PR_KT>(a, run, &g)) {
+        while (attn_next<C::ROWS, PR_KT, PR_OV>(a, run, &g)) {
             const int n = g.t1 - g.t0;
             if (n > 0) {
                 // ---- this warp's 32 rows of q, 128-byte swizzled; bf16 rows times a power of two that brings their
@@ -544,7 +545,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
             tc_fence_after();
             const uint32_t to = tl + C::o_col + t * DT;
             constexpr int PITCH = DT + 2;
-            float* part = a.part + attn_slot(run, g, blockIdx.x) * C::ROWS * PITCH;
+            float* part = a.part + attn_slot(g, blockIdx.x) * C::ROWS * PITCH;
             const float inv = g.whole ? (l == 0.f ? 0.f : __fdiv_rn(vs0, l)) : vs0;
             const bool live = M > -INFINITY || M != M || l != 0.f;   // rows that saw a key
             T* out = attn_out<T>(a, g, rr);
@@ -571,7 +572,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
             }
             tc_fence_before();   // O and S are read before the next item's MMAs, which this thread's arrivals release
             jj += max(n, 0);
-            if (!g.whole) attn_join<DT, C::ROWS, T>(a, run, g, stid, nsm, join_sh, bar);
+            if (!g.whole) attn_join<DT, C::ROWS, T>(a, g, stid, nsm, join_sh, bar);
         }
     }
     // The softmax warps have waited for the last O update, and so for every MMA, before tensor memory is freed

@@ -5,8 +5,8 @@
 //   O'_r = sum_j p'_jr c'_j,   l_r = sum_j p'_jr (V / vs_j),   o_r = V O'_r / l_r
 //
 // with codes c, c', one scale per page for K (ks) and V (vs), and V the largest vs so far. One persistent block per SM
-// (its run of units: attn_common.cuh), computing warps and a streaming one. The streaming warp brings, per unit of 64
-// keys, one TMA box of codes per page piece and 128-byte half for K and for V (128-byte swizzle), and the pages' scales
+// (its run of units: attn_common.cuh), computing warps and four streaming ones, which take the units in turn (one alone
+// issues a unit in about 700 cycles, 16 KB of the 44 GB/s that an SM can have). A streaming warp brings, per unit of 64 keys, one TMA box of codes per page piece and 128-byte half for K and for V (128-byte swizzle), and the pages' scales
 // with 4-byte asynchronous copies, into a ring of NS stages. Groups of four computing warps take the units in turn, 16
 // keys per warp, each warp with its own M and sums, joined once per segment.
 // Products are mma.sync.m16n8k16 on fp16 with the keys (or the dimensions) as the 16 rows and the queries as the 8
@@ -26,6 +26,8 @@
 namespace vkb {
 
 constexpr int AT_KT = 64;                            // keys per unit
+constexpr int TK_OV = 16;                            // an item's own cost in units
+constexpr int TK_STREAMS = 4;                        // streaming warps
 constexpr float TK_P_BIAS = 8.f;                     // p' is kept times 2^8
 
 // DT: head dimension rounded up to 64, 128 or 256. NQ: tiles of 8 query rows per item.
@@ -34,7 +36,7 @@ template <int DT, int NQ> struct TkCfg {
     static constexpr int OREG = DT * NQ / 4;                  // accumulator registers of a thread
     static constexpr int WARPS = OREG <= 32 ? 16 : 8;         // computing warps (groups of four)
     static constexpr int GROUPS = WARPS / 4;
-    static constexpr int THREADS = 32 * (WARPS + 4);          // and a warpgroup whose first warp streams
+    static constexpr int THREADS = 32 * (WARPS + 4);          // and the streaming warpgroup
     // registers: launched with LREG per thread; the streaming warpgroup keeps PREG, the computing ones have CREG
     static constexpr int LREG = WARPS == 16 ? 96 : 168, PREG = WARPS == 16 ? 32 : 40, CREG = WARPS == 16 ? 112 : 232;
     static_assert(128 * PREG + 32 * WARPS * CREG <= THREADS * LREG, "the split is of what the block is launched with");
@@ -42,7 +44,10 @@ template <int DT, int NQ> struct TkCfg {
     static constexpr int HB = DT < 128 ? DT : 128;            // bytes of a box row
     static constexpr int TILE = AT_KT * DT;                   // bytes of one tensor's codes in a stage
     static constexpr int STAGE = 2 * TILE;
-    static constexpr int NS = DT == 64 ? 16 : DT == 128 ? 10 : 5;
+    // Stages: a multiple of the streams and the groups, so that a stage always has the same streaming warp and the same
+    // group, which take its units in order (a barrier's phase can be waited for only until the next one completes).
+    static constexpr int NS = DT == 64 ? 16 : DT == 128 ? 8 : 4;
+    static_assert(NS % TK_STREAMS == 0 && TK_STREAMS % GROUPS == 0, "stages belong to a stream and a group");
     static constexpr int Q = QREGS ? 0 : ROWS * DT * 2;       // q in B-fragment order
     static constexpr int MERGE = WARPS * 8 * 64 * 4;          // 64 columns of 8 rows of every warp
     // offsets from the 1024-aligned base
@@ -53,7 +58,7 @@ template <int DT, int NQ> struct TkCfg {
     static constexpr int sc_off = row_off + ROWS * 4;         // [NS][4 pieces]{k, v} scales
     static constexpr int bar_off = (sc_off + NS * 32 + 15) / 16 * 16;
     static constexpr int run_off = bar_off + 16 * NS;
-    static constexpr int BYTES = run_off + 8 * (THREADS / 32 + 2) + 16 + 1024;
+    static constexpr int BYTES = run_off + 4 * (THREADS / 32 + 2) + 16 + 1024;
 };
 
 __device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
@@ -151,7 +156,7 @@ attn_token_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     uint64_t* full = reinterpret_cast<uint64_t*>(sm + C::bar_off);
     uint64_t* empty = full + C::NS;
     float* scales = reinterpret_cast<float*>(sm + C::sc_off);
-    long long* run_sh = reinterpret_cast<long long*>(sm + C::run_off);
+    unsigned* run_sh = reinterpret_cast<unsigned*>(sm + C::run_off);
     volatile int* join_sh = reinterpret_cast<volatile int*>(run_sh + C::THREADS / 32 + 2);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -166,20 +171,21 @@ attn_token_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         prefetch_tmap(&tv);
     }
     pdl_wait();
-    AttnRun run = attn_run<C::ROWS, AT_KT, C::THREADS>(a, run_sh);   // its barriers also publish the mbarriers
+    AttnRun run = attn_run<C::ROWS, AT_KT, TK_OV, C::THREADS>(a, run_sh);   // its barriers also publish the mbarriers
     AttnSeg g;
 
     if (warp >= C::WARPS) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::PREG));
-        if (warp > C::WARPS) return;
+        const int stream = warp - C::WARPS;
         // ===================== producer =====================
         const int pb = min(AT_KT, 1 << a.page_log2);   // keys per box
         int it = 0;
         bool ok = true;
-        while (ok && attn_next<C::ROWS, AT_KT>(a, run, &g)) {
+        while (ok && attn_next<C::ROWS, AT_KT, TK_OV>(a, run, &g)) {
             const int32_t* row = a.table + (long long)g.b * a.table_ld;
             int have = -1, ids = -1;   // this lane's page id of pages [have, have + 32)
             for (int t = g.t0; t < g.t1; ++t, ++it) {
+                if ((it & (TK_STREAMS - 1)) != stream) continue;
                 const int st = it % C::NS;
                 if (it >= C::NS) ok = __all_sync(0xffffffffu, wait_parity_sleep(&empty[st], (it / C::NS - 1) & 1));
                 if (!ok) break;
@@ -216,9 +222,9 @@ attn_token_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
                 __syncwarp();
             }
         }
-        // drain: every copy has landed before the block exits
+        // drain: every copy of this warp has landed before it exits
         for (int i = max(0, it - C::NS); i < it; ++i)
-            if (!wait_parity_sleep(&full[i % C::NS], (i / C::NS) & 1, DEV_ERR_DRAIN_TIMEOUT)) break;
+            if ((i & (TK_STREAMS - 1)) == stream && !wait_parity_sleep(&full[i % C::NS], (i / C::NS) & 1, DEV_ERR_DRAIN_TIMEOUT)) break;
         asm volatile("cp.async.wait_all;" ::: "memory");
         return;
     }
@@ -236,7 +242,7 @@ attn_token_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     float* rowf = reinterpret_cast<float*>(sm + C::row_off);
     int it = 0;
     bool ok = true;
-    while (attn_next<C::ROWS, AT_KT>(a, run, &g)) {
+    while (attn_next<C::ROWS, AT_KT, TK_OV>(a, run, &g)) {
         // ---- q: registers of every warp, or shared memory ----
         uint2 qr[C::QREGS ? KS : 1];
         float qf[NQ][2];   // scale * log2(e) over the factor of this thread's queries 8 nq + 2 qc + {0, 1}
@@ -430,7 +436,7 @@ attn_token_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         bar();
         const bool direct = g.whole;
         constexpr int PITCH = DT + 2;
-        float* part = a.part + attn_slot(run, g, blockIdx.x) * C::ROWS * PITCH;
+        float* part = a.part + attn_slot(g, blockIdx.x) * C::ROWS * PITCH;
 #pragma unroll
         for (int nq = 0; nq < NQ; ++nq) {
             float fac[2];
@@ -438,12 +444,12 @@ attn_token_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             for (int e = 0; e < 2; ++e) {
                 const int r = 8 * nq + 2 * qc + e;
                 float mm = -INFINITY, lsum = 0.f;
-#pragma unroll
+#pragma unroll 8
                 for (int w = 0; w < C::WARPS; ++w) mm = fmaxf(mm, ml[w * C::ROWS + r].x);
-#pragma unroll
+#pragma unroll 8
                 for (int w = 0; w < C::WARPS; ++w) {
                     const float2 v = ml[w * C::ROWS + r];
-                    if (v.x > -INFINITY) lsum = fmaf(v.y, ex2(v.x - mm), lsum);
+                    lsum = fmaf(v.y, ex2(v.x - (mm == -INFINITY ? 0.f : mm)), lsum);   // a warp that saw no key: 0
                 }
                 fac[e] = M[nq][e] > -INFINITY ? ex2(M[nq][e] - mm) * V : 0.f;
                 if (direct) fac[e] = lsum == 0.f ? 0.f : __fdiv_rn(fac[e], lsum);
@@ -483,7 +489,7 @@ attn_token_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
                 bar();
             }
         }
-        if (!direct) attn_join<DT, C::ROWS, T>(a, run, g, threadIdx.x, NT, join_sh, bar);
+        if (!direct) attn_join<DT, C::ROWS, T>(a, g, threadIdx.x, NT, join_sh, bar);
     }
 }
 
