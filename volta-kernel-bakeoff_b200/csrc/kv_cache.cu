@@ -11,8 +11,11 @@
 // (page, head, tensor) belongs to one block of threads, so nothing is atomic and the result does not depend on order.
 // Infinities are held as +-127 and do not enter the scale; NaN is held as 0.
 //
-// HBM-bound for prompts (every element read once, q written once, codes written once; the second pass over k and v
-// comes from L1 / L2), latency-bound for single tokens: one launch for q, k and v, blocks of 128 threads.
+// HBM-bound for prompts (every element read once, q written once, codes written once; a token's cosines are made once per
+// block and the turned k of a page stays in shared memory between the search for its maximum and its codes),
+// latency-bound for single tokens: one launch for q, k and v, blocks of 128 threads.
+#include <mutex>
+
 #include "step.cuh"
 
 namespace vkb {
@@ -32,6 +35,7 @@ struct AppendArgs {
     const void* kv[2];
     long long ldq, ldqo, ldkv[2];
     int pages, heads, page, dim, table_ld, B, T, hq, half_rot, layout, items;
+    int cs_max, cs_tokens, val_tokens;   // shared memory: cosines in all, of how many tokens; values of how many tokens
     float mscale;
 };
 
@@ -46,9 +50,10 @@ __device__ __forceinline__ float2 rope_cs(const AppendArgs& a, long long p, int 
     return make_float2(c * a.mscale, s * a.mscale);
 }
 
-// The rotated element e of a head whose elements start at p (turn: this tensor is rotated).
+// The rotated element e of a head whose elements start at p (turn: this tensor is rotated). cs: the token's cosines and
+// sines.
 template <int DT>
-__device__ __forceinline__ float rope_elem(const AppendArgs& a, const typename Elem<DT>::T* p, int e, long long pos,
+__device__ __forceinline__ float rope_elem(const AppendArgs& a, const typename Elem<DT>::T* p, int e, const float2* csp,
                                            bool turn) {
     const float v = Elem<DT>::to(p[e]);
     if (!turn || e >= 2 * a.half_rot) return v;
@@ -57,18 +62,18 @@ __device__ __forceinline__ float rope_elem(const AppendArgs& a, const typename E
     const bool second = half ? e >= a.half_rot : (e & 1) != 0;
     const int o = half ? (second ? e - a.half_rot : e + a.half_rot) : e ^ 1;
     const float w = Elem<DT>::to(p[o]);
-    const float2 cs = rope_cs(a, pos, i);
+    const float2 cs = csp[i];
     return second ? fmaf(v, cs.x, w * cs.y) : fmaf(v, cs.x, -w * cs.y);
 }
 
 // Eight consecutive elements e0.. of a head, rotated. vec: p is 16-byte aligned and the rotated part is made of whole
 // vectors (half layout: half_rot % 8 == 0; interleaved: half_rot % 4 == 0), so a vector lies in one part.
 template <int DT>
-__device__ __forceinline__ void rope_vec(const AppendArgs& a, const typename Elem<DT>::T* p, int e0, long long pos,
+__device__ __forceinline__ void rope_vec(const AppendArgs& a, const typename Elem<DT>::T* p, int e0, const float2* csp,
                                          bool turn, bool vec, float (&f)[8]) {
     if (!vec) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = rope_elem<DT>(a, p, e0 + e, pos, turn);
+        for (int e = 0; e < 8; ++e) f[e] = rope_elem<DT>(a, p, e0 + e, csp, turn);
         return;
     }
     Raw8<DT> r, o;
@@ -86,14 +91,14 @@ __device__ __forceinline__ void rope_vec(const AppendArgs& a, const typename Ele
         raw8_to<DT>(o, g);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float2 cs = rope_cs(a, pos, i0 + e);
+            const float2 cs = csp[i0 + e];
             f[e] = fmaf(f[e], cs.x, second ? g[e] * cs.y : -g[e] * cs.y);
         }
     } else {
         raw8_to<DT>(r, f);
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
-            const float2 cs = rope_cs(a, pos, (e0 + e) >> 1);
+            const float2 cs = csp[(e0 + e) >> 1];
             const float x = f[e], y = f[e + 1];
             f[e] = fmaf(x, cs.x, -y * cs.y);
             f[e + 1] = fmaf(y, cs.x, x * cs.y);
@@ -135,6 +140,7 @@ template <int DT> __global__ void __launch_bounds__(AP_THREADS) rope_append_kern
     using T = typename Elem<DT>::T;
     __shared__ int sh[AP_THREADS / 32 + 4];
     __shared__ float red[AP_THREADS / 32];
+    extern __shared__ __align__(16) uint8_t ap_smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     pdl_trigger();
     pdl_wait();
@@ -163,6 +169,9 @@ template <int DT> __global__ void __launch_bounds__(AP_THREADS) rope_append_kern
             if (t < s.q0 || t >= s.q0 + s.n) return;
             pos = (long long)s.len - s.n + (t - s.q0);
         }
+        float2* cs = reinterpret_cast<float2*>(ap_smem);
+        for (int i = tid; i < a.half_rot; i += AP_THREADS) cs[i] = rope_cs(a, pos, i);
+        __syncthreads();
         const T* q = reinterpret_cast<const T*>(a.q) + t * a.ldq;
         T* qo = reinterpret_cast<T*>(a.qo) + t * a.ldqo;
         const bool vin = rot_ok && aligned_to(a.q, 16) && (a.ldq * sizeof(T)) % 16 == 0;
@@ -178,7 +187,7 @@ template <int DT> __global__ void __launch_bounds__(AP_THREADS) rope_append_kern
                 const T* p = q + h * a.dim;
                 T* o = qo + h * a.dim;
                 if (e < a.half_rot) {
-                    const float x = rope_elem<DT>(a, p, e, pos, true), y = rope_elem<DT>(a, p, e + a.half_rot, pos, true);
+                    const float x = rope_elem<DT>(a, p, e, cs, true), y = rope_elem<DT>(a, p, e + a.half_rot, cs, true);
                     o[e] = Elem<DT>::from(x);
                     o[e + a.half_rot] = Elem<DT>::from(y);
                 } else {
@@ -194,8 +203,8 @@ template <int DT> __global__ void __launch_bounds__(AP_THREADS) rope_append_kern
             T* o = qo + h * a.dim;
             const int e0 = 8 * (j < hv ? j : j + hv);
             float f[8], g[8];
-            if (j < hv) rope_vec<DT>(a, p, e0 + a.half_rot, pos, true, true, g);
-            rope_vec<DT>(a, p, e0, pos, a.half_rot > 0, vin, f);
+            if (j < hv) rope_vec<DT>(a, p, e0 + a.half_rot, cs, true, true, g);
+            rope_vec<DT>(a, p, e0, cs, a.half_rot > 0, vin, f);
             if (vout) {
                 store8<DT>(o + e0, f);
                 if (j < hv) store8<DT>(o + e0 + a.half_rot, g);
@@ -273,16 +282,37 @@ template <int DT> __global__ void __launch_bounds__(AP_THREADS) rope_append_kern
     const long long ph = (long long)id * a.heads + h;
     uint8_t* codes = a.codes[which] + ph * a.page * a.dim;
     const float before = held > 0 ? a.scale[which][ph] : 0.f;
-    const int work = (hi - lo) * dv;
-    float amax = 0.f;
-    for (int i = tid; i < work; i += AP_THREADS) {
-        const int t = i / dv, e0 = 8 * (i - t * dv), row = s.q0 + (lo + t - p0);
-        const long long pos = a.pos ? a.pos[row] : lo + t;
-        float f[8];
-        rope_vec<DT>(a, src + row * ld, e0, pos, turn, vsrc, f);
+    // The tokens in turns of as many as shared memory holds, as fp32 (turned, for k): one turn but for the largest pages
+    // in fp32 rows of 128 x 256; where there is more than one, the second pass makes its values again.
+    const int count = hi - lo, dv4 = a.dim + 4;   // 4 floats apart from a multiple of the banks
+    float2* cs = reinterpret_cast<float2*>(ap_smem);
+    float* vals = reinterpret_cast<float*>(ap_smem + 8 * a.cs_max);
+    auto fill = [&](int t0, int n, float amax) {   // tokens t0 .. t0 + n - 1 into vals; their largest magnitude
+        for (int c0 = 0; c0 < n; c0 += a.cs_tokens) {
+            const int cn = min(a.cs_tokens, n - c0);
+            if (turn) {
+                __syncthreads();
+                for (int i = tid; i < cn * a.half_rot; i += AP_THREADS) {
+                    const int t = i / a.half_rot, row = s.q0 + (lo + t0 + c0 + t - p0);
+                    cs[i] = rope_cs(a, a.pos ? a.pos[row] : lo + t0 + c0 + t, i - t * a.half_rot);
+                }
+                __syncthreads();
+            }
+            for (int i = tid; i < cn * dv; i += AP_THREADS) {
+                const int t = i / dv, e0 = 8 * (i - t * dv), row = s.q0 + (lo + t0 + c0 + t - p0);
+                float f[8];
+                rope_vec<DT>(a, src + row * ld, e0, cs + t * a.half_rot, turn, vsrc, f);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_abs(f[e]));
-    }
+                for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_abs(f[e]));
+                float4* v = reinterpret_cast<float4*>(vals + (c0 + t) * dv4 + e0);
+                v[0] = make_float4(f[0], f[1], f[2], f[3]);
+                v[1] = make_float4(f[4], f[5], f[6], f[7]);
+            }
+        }
+        return amax;
+    };
+    float amax = 0.f;
+    for (int t0 = 0; t0 < count; t0 += a.val_tokens) amax = fill(t0, min(a.val_tokens, count - t0), amax);
     amax = warp_max(amax);
     if (lane == 0) red[warp] = amax;
     __syncthreads();   // also: every thread has read the old scale
@@ -309,15 +339,23 @@ template <int DT> __global__ void __launch_bounds__(AP_THREADS) rope_append_kern
             c[i] = make_uint2(w[0], w[1]);
         }
     }
-    for (int i = tid; i < work; i += AP_THREADS) {
-        const int t = i / dv, e0 = 8 * (i - t * dv), row = s.q0 + (lo + t - p0);
-        const long long pos = a.pos ? a.pos[row] : lo + t;
-        float f[8];
-        rope_vec<DT>(a, src + row * ld, e0, pos, turn, vsrc, f);
-        uint32_t c[2] = {0u, 0u};
+    for (int t0 = 0; t0 < count; t0 += a.val_tokens) {
+        const int n = min(a.val_tokens, count - t0);
+        if (count > a.val_tokens) {
+            __syncthreads();
+            fill(t0, n, 0.f);
+        }
+        __syncthreads();
+        for (int i = tid; i < n * dv; i += AP_THREADS) {
+            const int t = i / dv, e0 = 8 * (i - t * dv);
+            const float4* v = reinterpret_cast<const float4*>(vals + t * dv4 + e0);
+            const float4 x = v[0], y = v[1];
+            const float f[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+            uint32_t c[2] = {0u, 0u};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) c[e >> 2] |= kv_code(f[e], after) << (8 * (e & 3));
-        *reinterpret_cast<uint2*>(codes + (held + t) * a.dim + e0) = make_uint2(c[0], c[1]);
+            for (int e = 0; e < 8; ++e) c[e >> 2] |= kv_code(f[e], after) << (8 * (e & 3));
+            *reinterpret_cast<uint2*>(codes + (held + t0 + t) * a.dim + e0) = make_uint2(c[0], c[1]);
+        }
     }
 }
 
@@ -329,39 +367,33 @@ struct ReadArgs {
     int pages, heads, page, dim, table_ld, B, n;
 };
 
-// One thread: 16 codes (one 16-byte load) of one token and head.
+// A warp takes a token's heads and dimensions by 256 codes, eight per lane (an 8-byte load, a 16-byte store of 16-bit
+// values: both contiguous over the warp).
 template <int DT> __global__ void __launch_bounds__(256) kv_read_kernel(const ReadArgs a) {
     using T = typename Elem<DT>::T;
     pdl_trigger();
     pdl_wait();
-    const int per = a.dim >> 4;
-    const long long total = (long long)a.n * a.heads * per;
-    const int which = blockIdx.y;
-    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
-        const int c = (int)(i % per);
-        const long long th = i / per;
-        const int t = (int)(th / a.heads), h = (int)(th - (long long)t * a.heads);
+    const int which = blockIdx.y, lane = threadIdx.x & 31, warps = gridDim.x * 8, per = a.dim >> 3, all = a.heads * per;
+    for (int t = blockIdx.x * 8 + (threadIdx.x >> 5); t < a.n; t += warps) {
         const int b = a.seq[t], p = a.pos[t];
-        T* out = reinterpret_cast<T*>(a.out[which]) + th * a.dim + 16 * c;
-        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, g[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         bool ok = b >= 0 && b < a.B && p >= 0 && p < (long long)a.table_ld * a.page;
         const int id = ok ? a.table[(long long)b * a.table_ld + p / a.page] : -1;
         ok = ok && id >= 0 && id < a.pages;
-        if (ok) {
-            const long long ph = (long long)id * a.heads + h;
-            const uint4 v = *reinterpret_cast<const uint4*>(a.codes[which] + (ph * a.page + p % a.page) * a.dim + 16 * c);
-            const float s = a.scale[which][ph];
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        if (!ok && lane == 0) raise_status(DEV_ERR_BAD_INDEX);   // a token that is not in the table reads as zeros
+        T* out = reinterpret_cast<T*>(a.out[which]) + (long long)t * a.heads * a.dim;
+        for (int i = lane; i < all; i += 32) {
+            const int h = i / per, e0 = 8 * (i - h * per);
+            float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            if (ok) {
+                const long long ph = (long long)id * a.heads + h;
+                const uint2 v = *reinterpret_cast<const uint2*>(a.codes[which] + (ph * a.page + p % a.page) * a.dim + e0);
+                const float s = a.scale[which][ph];
+                const uint32_t w[2] = {v.x, v.y};
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                f[e] = (float)((int)((w[e >> 2] >> (8 * (e & 3))) & 255u) - 128) * s;
-                g[e] = (float)((int)((w[2 + (e >> 2)] >> (8 * (e & 3))) & 255u) - 128) * s;
+                for (int e = 0; e < 8; ++e) f[e] = (float)((int)((w[e >> 2] >> (8 * (e & 3))) & 255u) - 128) * s;
             }
-        } else {
-            raise_status(DEV_ERR_BAD_INDEX);   // a token that is not in the table reads as zeros
+            store8<DT>(out + 8 * i, f);
         }
-        store8<DT>(out, f);
-        store8<DT>(out + 8, g);
     }
 }
 
@@ -411,9 +443,25 @@ extern "C" int vkb_rope_append(const vkb_kv_cache_t* c, const int32_t* table, in
     a.pages = c->pages; a.heads = c->heads; a.page = c->page; a.dim = c->dim; a.table_ld = table_ld;
     a.B = B; a.T = T; a.hq = q_heads; a.half_rot = rot / 2; a.layout = layout; a.items = (int)items;
     a.mscale = mscale;
+    // Shared memory of a block: cosines and sines of 1024 pairs (or one token's), values of a page's tokens up to 40 KB (five
+    // blocks per SM); single tokens take what one needs.
+    const int pairs = rot / 2 > 0 ? rot / 2 : 1, value = 4 * (c->dim + 4);
+    a.cs_tokens = !cu ? 1 : 1024 / pairs > 1 ? 1024 / pairs : 1;
+    if (a.cs_tokens > c->page) a.cs_tokens = c->page;
+    a.cs_max = (a.cs_tokens * pairs + 1) / 2 * 2;
+    a.val_tokens = !cu ? 1 : 40960 / value < c->page ? 40960 / value : c->page;
+    const size_t smem = 8 * (size_t)a.cs_max + (size_t)a.val_tokens * value;
     auto kern = dt == VKB_DT_F16 ? rope_append_kernel<VKB_DT_F16>
                 : dt == VKB_DT_BF16 ? rope_append_kernel<VKB_DT_BF16> : rope_append_kernel<VKB_DT_F32>;
-    return launch_pdl(kern, dim3((unsigned)grid), dim3(AP_THREADS), 0, (cudaStream_t)stream, 1, a);
+    static std::once_flag once[kMaxDevices][3];
+    static cudaError_t err[kMaxDevices][3];
+    int dev = 0;
+    if (int r = current_device(&dev)) return r;
+    std::call_once(once[dev][dt], [&] {
+        err[dev][dt] = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 8 * 1024 + 40960);
+    });
+    if (err[dev][dt] != cudaSuccess) return -(int)err[dev][dt];
+    return launch_pdl(kern, dim3((unsigned)grid), dim3(AP_THREADS), smem, (cudaStream_t)stream, 1, a);
 }
 
 extern "C" int vkb_kv_read(const vkb_kv_cache_t* c, const int32_t* table, int table_ld, int B, const int32_t* seq,
@@ -424,7 +472,7 @@ extern "C" int vkb_kv_read(const vkb_kv_cache_t* c, const int32_t* table, int ta
     if (!seq || !pos || !k || !v || !aligned_to(k, 16) || !aligned_to(v, 16)) return VKB_EINVAL;
     const ReadArgs a{{(const uint8_t*)c->k, (const uint8_t*)c->v}, {c->k_scale, c->v_scale}, {k, v}, table, seq, pos,
                      c->pages, c->heads, c->page, c->dim, table_ld, B, n};
-    const long long want = ((long long)n * c->heads * (c->dim / 16) + 255) / 256;
+    const long long want = ((long long)n + 7) / 8;
     const dim3 grid((unsigned)(want < 148 * 16 ? want : 148 * 16), 2);
     auto kern = dt == VKB_DT_F16 ? kv_read_kernel<VKB_DT_F16>
                 : dt == VKB_DT_BF16 ? kv_read_kernel<VKB_DT_BF16> : kv_read_kernel<VKB_DT_F32>;
