@@ -5,8 +5,8 @@
 // rows of the tile. The scales never touch the codes: with x_j = s_j ks_j scale log2(e) + log2(vs_j / vs0),
 //   p'_j = 2^(x_j - M + 8),   O' = sum_j p'_j c'_j,   l = sum_j p'_j (vs0 / vs_j),   o = vs0 O' / l,
 // so a group of 16 keys (a page or part of one) costs one multiply-add per score and one multiply per group. p' is
-// rounded once, to fp16, for the product; l sums it in fp32. M follows the running maximum of x lazily (by up to 2^4), so
-// O' is rescaled only when a row's maximum grows by more. vs0: the largest V scale of the segment's first keys; scales
+// rounded once, to fp16, for the product; l sums it in fp32. M follows the running maximum of x lazily, so that O' is
+// rescaled only when a p' might leave fp16's range. vs0: the largest V scale of the segment's first keys; scales
 // below 2^-30 of the largest seen so far count as that.
 //
 // 16 warps, one block per SM (its run of units: attn_common.cuh):
@@ -130,9 +130,9 @@ __device__ __forceinline__ float pr_max(const uint32_t (&s)[32], const float4* s
     }
     return mx;
 }
-// p' of 32 scores as fp16 pairs, and their sum into l (two running halves).
+// p' of 32 scores as fp16 pairs, their sum into l (two running halves), and into top the largest sum of eight of them.
 __device__ __forceinline__ void pr_exp(const uint32_t (&s)[32], uint32_t (&pk)[16], const float4* sc, float qinv, float mb,
-                                       uint64_t& l) {
+                                       uint64_t& l, float& top) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const float4 f = sc[h];
@@ -148,7 +148,10 @@ __device__ __forceinline__ void pr_exp(const uint32_t (&s)[32], uint32_t (&pk)[1
             sum[(e >> 1) & 1] = e < 4 ? p : f2_add(sum[(e >> 1) & 1], p);
             pk[8 * h + e / 2] = pack_f16(x.x, x.y);
         }
-        l = f2_fma(f2_add(sum[0], sum[1]), f2_make(f.z, f.z), l);
+        const uint64_t both = f2_add(sum[0], sum[1]);
+        const float2 b = f2_get(both);
+        top = max3(top, b.x, b.y);
+        l = f2_fma(both, f2_make(f.z, f.z), l);
     }
 }
 
@@ -490,21 +493,18 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
                 };
                 vs0 = sc[0].w;
                 read();
-                // ---- p' against the M of the tiles before this one, and its sum. Where a row's largest p' passes 2^(8 + 4),
-                // M is moved up and the tile is done again: the first tile that a row sees, and few others, so that the
-                // maximum is taken on 32 packed pairs instead of 64 scores ahead of everything else ----
+                // ---- p' against the M of the tiles before this one, and its sum. Where eight p' of a row add up to more than
+                // 2^15 (so that one of them might pass fp16's 65504), M is moved up to the maximum and the tile is done
+                // again: the first tile that a row sees, and few others, so that the maximum of the scores is not taken
+                // ahead of everything else ----
                 uint32_t pk[16], pk2[16];
                 uint64_t sum = 0;
-                float mb = M == -INFINITY ? 0.f : M - PR_BIAS;
-                pr_exp(s, pk, sc, qinv, mb, sum);
-                pr_exp(s2, pk2, sc + 2, qinv, mb, sum);
-                uint32_t top = h2_max(pk[0], pk2[0]);
-#pragma unroll
-                for (int e = 1; e < 16; ++e) top = h2_max(top, h2_max(pk[e], pk2[e]));
-                // a row's first keys, or too large a p' in either half (fp16 4096 = 0x6c00; positive numbers order
-                // like integers; NaN, 0x7fff, counts as too large, is done again and stays NaN)
+                float mb = M == -INFINITY ? 0.f : M - PR_BIAS, top = 0.f;
+                pr_exp(s, pk, sc, qinv, mb, sum, top);
+                pr_exp(s2, pk2, sc + 2, qinv, mb, sum, top);
                 const bool unset = M == -INFINITY && klo < key0 + PR_KT && khi > key0;   // the row's first keys
-                if (__any_sync(0xffffffffu, unset || (top & 0xffffu) > 0x6c00u || (top >> 16) > 0x6c00u)) {
+                if (__any_sync(0xffffffffu, unset || top > 32768.f)) {
+                    read();   // again, so that the scores need not stay in registers meanwhile
                     const float mx = pr_max(s2, sc + 2, qinv, pr_max(s, sc, qinv, -INFINITY));
                     const float mn = fmaxf(M, mx), al = M == -INFINITY ? 0.f : ex2(M - mn);
                     M = mn;
@@ -524,8 +524,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
                     }
                     sum = 0;
                     mb = M == -INFINITY ? 0.f : M - PR_BIAS;
-                    pr_exp(s, pk, sc, qinv, mb, sum);
-                    pr_exp(s2, pk2, sc + 2, qinv, mb, sum);
+                    pr_exp(s, pk, sc, qinv, mb, sum, top);
+                    pr_exp(s2, pk2, sc + 2, qinv, mb, sum, top);
                 }
                 l2 = f2_add(l2, sum);
                 tmem_st16(ts, pk);   // in place of S's first 32 columns
