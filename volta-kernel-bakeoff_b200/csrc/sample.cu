@@ -24,7 +24,8 @@ namespace vkb {
 
 constexpr int SM_THREADS = 512;
 constexpr int SM_NB = 1024;      // bins
-constexpr int SM_CAP = 1024;     // tokens of a boundary bin that are ranked directly
+constexpr int SM_CAP = 128;      // tokens of a boundary bin that are ranked directly (each against all: at 1024 the ranking of
+                                 // a crowded bin, 600 tokens in 150000, took longer than splitting the bin)
 constexpr float SM_SPAN = 46.f;  // bins cover distances up to this, in powers of two (the last bin: everything beyond)
 constexpr int SM_LOCAL = 2048;   // candidates for the first block that one block can hold
 constexpr int SM_MAX_SLICE = 49152;   // floats of a row that one block holds
@@ -149,11 +150,15 @@ __device__ __noinline__ int sm_find(SmShared* s, const SmRow& row, bool by_count
     }
     unsigned ci = csum;
     double mi = msum;
+    const bool mass = !by_count || edge >= 0.f;   // the block together
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const unsigned p = __shfl_up_sync(0xffffffffu, ci, o);
-        const double q = __shfl_up_sync(0xffffffffu, mi, o);
-        if (lane >= o) { ci += p; mi += q; }
+        if (lane >= o) ci += p;
+        if (mass) {
+            const double q = __shfl_up_sync(0xffffffffu, mi, o);
+            if (lane >= o) mi += q;
+        }
     }
     if (lane == 31) { s->scan_n[warp] = ci; s->scan[warp] = mi; }
     if (tid == 0) s->out_i = SM_NB;
@@ -162,8 +167,11 @@ __device__ __noinline__ int sm_find(SmShared* s, const SmRow& row, bool by_count
     double mb = 0.0, all = 0.0;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
-        if (w < warp) { cb += s->scan_n[w]; mb += s->scan[w]; }
-        all += s->scan[w];
+        if (w < warp) cb += s->scan_n[w];
+        if (mass) {
+            if (w < warp) mb += s->scan[w];
+            all += s->scan[w];
+        }
     }
     cb += ci - csum;
     mb += mi - msum;
@@ -408,12 +416,10 @@ __device__ __noinline__ double sm_boundary(SmShared* s, const SmSlice& z, const 
     return cm;
 }
 
-// All blocks: cut the order and take the token.
+// All blocks: the last token that top-k and top-p keep, by histograms.
 template <int CL>
-__device__ __forceinline__ void sm_finish(SmShared* s, const SmSlice& z, const SmRow& row, int k, int held, float tp,
-                                          float mp, float u, int32_t* token, float* prob) {
+__device__ __forceinline__ SmEntry sm_cut(SmShared* s, const SmSlice& z, const SmRow& row, int k, int held, float tp) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int rank = CL > 1 ? (int)cluster_ctarank() : 0;
     const bool by_k = k > 1 && k < held, by_p = tp < 1.f;
     SmEntry cut{-INFINITY, 0x7fffffff};   // keep everything
     if (by_k || by_p) {
@@ -461,68 +467,90 @@ __device__ __forceinline__ void sm_finish(SmShared* s, const SmSlice& z, const S
             cut = pcut.l > kcut.l || (pcut.l == kcut.l && pcut.i < kcut.i) ? pcut : kcut;
         }
     }
+    return cut;
+}
+
+// All blocks: the token among those down to `cut` that weigh at least mp of the largest.
+template <int CL>
+__device__ __forceinline__ void sm_take(SmShared* s, const SmSlice& z, const SmRow& row, SmEntry cut, float mp, float u,
+                                        int32_t* token, float* prob) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rank = CL > 1 ? (int)cluster_ctarank() : 0;
     // ---- the kept weight, by warp (contiguous pieces), block and row ----
     const float floor_w = fminf(mp, 1.f);
     auto kept = [&](int i) {   // weight of token i, 0 where it is not kept
-        const float l = z.x[i];
-        if (l < cut.l || (l == cut.l && z.index(i) > cut.i)) return 0.f;
-        const float w = sm_weight(sm_dist(row, l));
-        return w >= floor_w ? w : 0.f;
+        const float l = z.x[i], w = sm_weight(sm_dist(row, l));
+        const bool in = l > cut.l || (l == cut.l && (cut.i == 0x7fffffff || z.index(i) <= cut.i));
+        return in && w >= floor_w ? w : 0.f;
     };
     constexpr int nw = SM_THREADS / 32;
     const int piece = (z.n0 + nw - 1) / nw, i0 = min(z.n0, warp * piece), i1 = min(z.n0, i0 + piece);
     float part = 0.f;
+#pragma unroll 4
     for (int i = i0 + lane; i < i1; i += 32) part += kept(i);
     part = warp_sum(part);
     if (lane == 0) s->wsum[warp] = (double)part;
     __syncthreads();
-    double own = 0.0;
+    double mine = 0.0, own = 0.0;   // warp 0: lane i has warp i's weight, and the block's
+    if (warp == 0) {
+        mine = lane < nw ? s->wsum[lane] : 0.0;
+        own = mine;
 #pragma unroll
-    for (int w = 0; w < nw; ++w) own += s->wsum[w];
+        for (int o = 16; o; o >>= 1) own += __shfl_xor_sync(0xffffffffu, own, o);
+    }
     double ahead = 0.0, total = own;
     int last = 0;   // the last block with any weight
     if constexpr (CL > 1) {
         if (tid == 0) s->sum = own;
         row_sync<CL>();
-        total = 0.0;
+        if (warp == 0) {
+            total = 0.0;
 #pragma unroll
-        for (int r = 0; r < CL; ++r) {
-            const double v = peer<CL>(&s->sum, r);
-            if (r < rank) ahead += v;
-            total += v;
-            if (v > 0.0) last = r;
+            for (int r = 0; r < CL; ++r) {
+                const double v = peer<CL>(&s->sum, r);
+                if (r < rank) ahead += v;
+                total += v;
+                if (v > 0.0) last = r;
+            }
         }
     }
     const double target = (double)u * total;
     // this block holds the token if the target falls into its part (the last one with weight takes rounding at the end)
-    if (own > 0.0 && ahead <= target && (target < ahead + own || rank == last) && warp == 0) {
-        int w = 0, lw = 0;
-        double m = ahead;
-        for (int j = 0; j < nw; ++j) if (s->wsum[j] > 0.0) lw = j;
-        while (w < lw && !(s->wsum[w] > 0.0 && target < m + s->wsum[w])) m += s->wsum[w++];
+    if (warp == 0 && own > 0.0 && ahead <= target && (target < ahead + own || rank == last)) {
+        double inc = mine;
+#pragma unroll
+        for (int o = 1; o < nw; o <<= 1) {
+            const double p = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += p;
+        }
+        // the warp's piece that the target falls into: the first that passes it, else the last with weight
+        const unsigned pass = __ballot_sync(0xffffffffu, mine > 0.0 && target < ahead + inc);
+        const unsigned any = __ballot_sync(0xffffffffu, mine > 0.0);
+        const int w = pass ? __ffs(pass) - 1 : 31 - __clz(any);
+        double m = ahead + __shfl_sync(0xffffffffu, inc - mine, w);
         const int a0 = min(z.n0, w * piece), a1 = min(z.n0, a0 + piece);
         int found = -1, back = -1;
         float fw = 0.f, bw = 0.f;
         for (int i = a0; i < a1 && found < 0; i += 32) {
             const float v = i + lane < a1 ? kept(i + lane) : 0.f;
-            float inc = v;
+            float run = v;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const float p = __shfl_up_sync(0xffffffffu, inc, o);
-                if (lane >= o) inc += p;
+                const float p = __shfl_up_sync(0xffffffffu, run, o);
+                if (lane >= o) run += p;
             }
-            const unsigned hit = __ballot_sync(0xffffffffu, v > 0.f && m + (double)inc > target);
-            const unsigned any = __ballot_sync(0xffffffffu, v > 0.f);
+            const unsigned hit = __ballot_sync(0xffffffffu, v > 0.f && m + (double)run > target);
+            const unsigned some = __ballot_sync(0xffffffffu, v > 0.f);
             if (hit) {
                 const int b = __ffs(hit) - 1;
                 found = i + b;
                 fw = __shfl_sync(0xffffffffu, v, b);
-            } else if (any) {
-                const int b = 31 - __clz(any);
+            } else if (some) {
+                const int b = 31 - __clz(some);
                 back = i + b;
                 bw = __shfl_sync(0xffffffffu, v, b);
             }
-            m += (double)__shfl_sync(0xffffffffu, inc, 31);
+            m += (double)__shfl_sync(0xffffffffu, run, 31);
         }
         if (found < 0) { found = back; fw = bw; }
         if (lane == 0) {
@@ -544,9 +572,6 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(const SampleArgs 
     const int first = rank * a.slice, n0 = max(0, min(a.slice, a.V - first));
     pdl_trigger();
     pdl_wait();
-    const float t = a.temperature ? a.temperature[rw] : 1.f, u = fminf(fmaxf(a.u[rw], 0.f), 1.f);   // NaN: 0
-    const int k = a.top_k ? a.top_k[rw] : 0;
-    const float tp = a.top_p ? a.top_p[rw] : 1.f, mp = a.min_p ? a.min_p[rw] : 0.f;
     // ---- read the slice; maximum (lowest index among equals), smallest finite logit ----
     const T* g = reinterpret_cast<const T*>(a.logits) + rw * a.ld + first;
     float hi = -INFINITY, lo = INFINITY;
@@ -585,6 +610,9 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(const SampleArgs 
         see(f, i);
         x[i] = f;
     }
+    const float t = a.temperature ? a.temperature[rw] : 1.f, u = fminf(fmaxf(a.u[rw], 0.f), 1.f);   // NaN: 0
+    const int k = a.top_k ? a.top_k[rw] : 0;
+    const float tp = a.top_p ? a.top_p[rw] : 1.f, mp = a.min_p ? a.min_p[rw] : 0.f;
     s->tmax[tid] = hi;
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
@@ -715,15 +743,18 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(const SampleArgs 
                     }
                 }
                 row_sync<CL>();   // the others leave
-                if (rank == 0)
-                    sm_finish<1>(s, SmSlice{x, list, count, 0}, row, k, a.V, tp, mp, u, a.token + rw,
-                                 a.prob ? a.prob + rw : nullptr);
+                if (rank == 0) {
+                    const SmSlice z{x, list, count, 0};
+                    const SmEntry cut = sm_cut<1>(s, z, row, k, a.V, tp);
+                    sm_take<1>(s, z, row, cut, mp, u, a.token + rw, a.prob ? a.prob + rw : nullptr);
+                }
                 return;
             }
             row_sync<CL>();   // the candidates' counts have been read
         }
     }
-    sm_finish<CL>(s, SmSlice{x, nullptr, n0, first}, row, k, a.V, tp, mp, u, a.token + rw, a.prob ? a.prob + rw : nullptr);
+    const SmSlice z{x, nullptr, n0, first};
+    sm_take<CL>(s, z, row, sm_cut<CL>(s, z, row, k, a.V, tp), mp, u, a.token + rw, a.prob ? a.prob + rw : nullptr);
     if constexpr (CL > 1) row_sync<CL>();
 }
 
