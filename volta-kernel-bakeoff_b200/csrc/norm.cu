@@ -24,7 +24,8 @@ struct NormArgs {
     int T, d;
 };
 
-constexpr int NORM_NV = 2;   // vectors of eight a thread holds (1024 threads x 2 x 8 = 16384 elements)
+constexpr int NORM_NV = 2;    // vectors of eight a thread holds (1024 threads x 2 x 8 = 16384 elements)
+constexpr int NORM_WNV = 10;  // and where a warp takes a row of its own (rows of up to 2560 elements)
 
 // Sum over the threads of one row: a warp, or the whole block (blockDim.y == 1).
 __device__ __forceinline__ float row_sum(float v, float* red) {
@@ -48,29 +49,31 @@ __device__ __forceinline__ int q8_code(float v, float inv) {
     return (int)fminf(127.f, fmaxf(-127.f, roundf(v * inv)));
 }
 
-template <int X, int R>   // element types of x / w / y and of the residual (R = -1: none)
-__global__ void __launch_bounds__(1024) norm_vec_kernel(const NormArgs a) {
+// X, R: element types of x / w / y and of the residual (R = -1: none). NV: vectors a thread holds; WARP: a row per warp,
+// whose weights are read when they are needed (the row itself fills the registers).
+template <int X, int R, int NV, bool WARP>
+__global__ void __launch_bounds__(WARP ? 128 : 1024) norm_vec_kernel(const NormArgs a) {
     using TX = typename Elem<X>::T;
     constexpr int RD = R < 0 ? 0 : R;
     using TR = typename Elem<RD>::T;
     __shared__ float red[32];
     const int row = blockIdx.x * blockDim.y + threadIdx.y;
-    const int nvec = a.d >> 3, tpr = blockDim.x;
+    const int nvec = a.d >> 3, tpr = WARP ? 32 : blockDim.x;
     pdl_trigger();
-    Raw8<X> w[NORM_NV];
+    Raw8<X> w[WARP ? 1 : NV];
 #pragma unroll
-    for (int j = 0; j < NORM_NV; ++j) {
+    for (int j = 0; j < NV; ++j) {
         const int i = threadIdx.x + j * tpr;
-        if (i < nvec) prefetch_l2(reinterpret_cast<const TX*>(a.w) + 8 * i);
+        if (!WARP && i < nvec) prefetch_l2(reinterpret_cast<const TX*>(a.w) + 8 * i);
     }
     pdl_wait();
     if (row >= a.T) return;   // whole warps: a row's threads leave together
     const TX* x = reinterpret_cast<const TX*>(a.x) + row * a.ldx;
     const long long base = (long long)row * a.d;
-    Raw8<X> rx[NORM_NV];
-    Raw8<RD> rr[NORM_NV];
+    Raw8<X> rx[NV];
+    Raw8<RD> rr[NV];
 #pragma unroll
-    for (int j = 0; j < NORM_NV; ++j) {
+    for (int j = 0; j < NV; ++j) {
         const int i = threadIdx.x + j * tpr;
         if (i < nvec) {
             raw8_load<X>(rx[j], x + 8 * i);
@@ -78,13 +81,13 @@ __global__ void __launch_bounds__(1024) norm_vec_kernel(const NormArgs a) {
         }
     }
 #pragma unroll
-    for (int j = 0; j < NORM_NV; ++j) {
+    for (int j = 0; j < NV; ++j) {
         const int i = threadIdx.x + j * tpr;
-        if (i < nvec) raw8_load<X>(w[j], reinterpret_cast<const TX*>(a.w) + 8 * i);
+        if (!WARP && i < nvec) raw8_load<X>(w[WARP ? 0 : j], reinterpret_cast<const TX*>(a.w) + 8 * i);
     }
-    float f[NORM_NV][8], ss = 0.f;
+    float f[NV][8], ss = 0.f;
 #pragma unroll
-    for (int j = 0; j < NORM_NV; ++j) {
+    for (int j = 0; j < NV; ++j) {
         const int i = threadIdx.x + j * tpr;
         if (i >= nvec) continue;
         raw8_to<X>(rx[j], f[j]);
@@ -101,13 +104,14 @@ __global__ void __launch_bounds__(1024) norm_vec_kernel(const NormArgs a) {
     ss = row_sum(ss, red);
     const float rs = __fdiv_rn(1.f, __fsqrt_rn(fmaf(ss, a.inv_d, a.eps)));
 #pragma unroll
-    for (int j = 0; j < NORM_NV; ++j) {
+    for (int j = 0; j < NV; ++j) {
         const int i = threadIdx.x + j * tpr;
         const bool on = i < nvec;
         float amax = 0.f;
         if (on) {
             float g[8];
-            raw8_to<X>(w[j], g);
+            if (WARP) raw8_load<X>(w[0], reinterpret_cast<const TX*>(a.w) + 8 * i);
+            raw8_to<X>(w[WARP ? 0 : j], g);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 f[j][e] = f[j][e] * rs * g[e];
@@ -174,10 +178,17 @@ __global__ void __launch_bounds__(1024) norm_any_kernel(const NormArgs a) {
 template <int X, int R> static int norm_launch(const NormArgs& a, bool vec, cudaStream_t st) {
     // threads per row: one vector (or element) each where that is at most 1024, a warp for short rows
     const int n = vec ? a.d / 8 : a.d;
+    // A warp per row where there are rows for every SM's warps: no block-wide barrier, and a row's loads all in flight at
+    // once (B200, bf16 in, residual and out: 8191 rows of 2560 take 34 us, 37 with a block per row; 2047 and 2048 rows 11 us
+    // either way).
+    if (vec && n > 64 && n <= 32 * NORM_WNV && a.T >= 2048) {
+        const dim3 grid((unsigned)((a.T + 3) / 4)), block(32, 4);
+        return launch_pdl(norm_vec_kernel<X, R, NORM_WNV, true>, grid, block, 0, st, 1, a);
+    }
     const int tpr = n <= 64 ? 32 : min(1024, (n + 31) / 32 * 32);
     const int rows = tpr == 32 ? 4 : 1;
     const dim3 grid((unsigned)((a.T + rows - 1) / rows)), block((unsigned)tpr, (unsigned)rows);
-    return launch_pdl(vec ? norm_vec_kernel<X, R> : norm_any_kernel<X, R>, grid, block, 0, st, 1, a);
+    return launch_pdl(vec ? norm_vec_kernel<X, R, NORM_NV, false> : norm_any_kernel<X, R>, grid, block, 0, st, 1, a);
 }
 
 template <int X> static int norm_res(const NormArgs& a, int res_dt, bool vec, cudaStream_t st) {
