@@ -449,6 +449,28 @@ def test_attention_streams_graphs_and_growth(cuda):
     del graph
 
 
+def test_tensors_of_another_stream(cuda):
+    """A call on another stream marks its tensors as used there: memory given back at once is not handed out again while
+    the call still waits for that stream's earlier work."""
+    import torch
+    x = torch.randn((4096, 2048), generator=gen(2), device="cuda").half()
+    w = torch.ones(2048, device="cuda").half()
+    want = vkb.rms_norm(x, w)[0]
+    torch.cuda.synchronize()
+    other = torch.cuda.Stream()
+    with torch.cuda.stream(other):
+        a = torch.randn((4096, 4096), device="cuda")
+        for _ in range(20):
+            a = a @ a * 1e-3
+    y = vkb.rms_norm(x, w, stream=other)[0]
+    ptr = x.data_ptr()
+    del x
+    z = torch.zeros((4096, 2048), dtype=torch.float16, device="cuda")
+    assert z.data_ptr() != ptr
+    torch.cuda.synchronize()
+    assert torch.equal(y, want)
+
+
 def test_attention_refusals(cuda):
     import torch
     cache, table, ln = make_cache([10], 2, 64, 16)

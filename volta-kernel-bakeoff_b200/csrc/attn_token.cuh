@@ -443,14 +443,16 @@ attn_token_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int r = 8 * nq + 2 * qc + e;
-                float mm = -INFINITY, lsum = 0.f;
-#pragma unroll 8
-                for (int w = 0; w < C::WARPS; ++w) mm = fmaxf(mm, ml[w * C::ROWS + r].x);
-#pragma unroll 8
-                for (int w = 0; w < C::WARPS; ++w) {
-                    const float2 v = ml[w * C::ROWS + r];
-                    lsum = fmaf(v.y, ex2(v.x - (mm == -INFINITY ? 0.f : mm)), lsum);   // a warp that saw no key: 0
-                }
+                // the eight lanes of a column pair take the warps' values between them
+                const float2 v0 = ml[gr * C::ROWS + r];
+                const float2 v1 = C::WARPS == 16 ? ml[((gr + 8) & (C::WARPS - 1)) * C::ROWS + r] : make_float2(-INFINITY, 0.f);
+                float mm = fmaxf(v0.x, v1.x);
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
+                const float mu = mm == -INFINITY ? 0.f : mm;   // a warp that saw no key: 0
+                float lsum = fmaf(v0.y, ex2(v0.x - mu), v1.y * ex2(v1.x - mu));
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) lsum += __shfl_xor_sync(0xffffffffu, lsum, d);
                 fac[e] = M[nq][e] > -INFINITY ? ex2(M[nq][e] - mm) * V : 0.f;
                 if (direct) fac[e] = lsum == 0.f ? 0.f : __fdiv_rn(fac[e], lsum);
                 if (!direct && warp == 0 && gr == 0 && r < g.rows)

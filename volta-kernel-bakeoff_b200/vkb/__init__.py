@@ -238,8 +238,11 @@ def _torch():
 
 def _stream(stream=None) -> ctypes.c_void_p:
     torch = _torch()
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return ctypes.c_void_p(s.cuda_stream)
+    if stream is not None:
+        return ctypes.c_void_p(stream.cuda_stream)
+    # the handle alone is a lookup; torch.cuda.current_stream() makes an object, 3 us per call on the host
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return ctypes.c_void_p(raw(torch.cuda.current_device()) if raw else torch.cuda.current_stream().cuda_stream)
 
 
 def _ptr(t) -> ctypes.c_void_p:

@@ -2,8 +2,8 @@
 into a paged 8-bit cache), attention over that cache, and sample. Torch tensors in and out; every call is one kernel
 of libvkb.so on the current stream (or `stream`), described in include/vkb.h.
 
-Outputs that are not given are allocated. With `stream` the inputs must be ready on that stream, and the outputs made
-here are allocated for it.
+Outputs that are not given are allocated. With `stream` the inputs must be ready on that stream; outputs made here are
+allocated for it, and the allocator is told that the tensors given are in use on it.
 """
 from __future__ import annotations
 
@@ -65,6 +65,14 @@ def _new(like, shape, dtype, stream):
         return like.new_empty(shape, dtype=dtype)
 
 
+def _used(stream, *tensors) -> None:
+    """Tensors of a call on a stream that need not be their own: their memory is not reused before the call has run."""
+    if stream is not None:
+        for t in tensors:
+            if t is not None:
+                t.record_stream(stream)
+
+
 def _p(t):
     return None if t is None else t.data_ptr()
 
@@ -111,6 +119,7 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6, y=None, residual_out=N
         q, s = _new(x, (T, d), torch.int8, stream), _new(x, (T, d // 32), torch.float16, stream)
     check(lib().vkb_rms_norm(dt, x.data_ptr(), x.stride(0) if T > 1 else d, _p(residual), _p(residual_out), res_dt,
                              weight.data_ptr(), eps, y.data_ptr(), _p(q), _p(s), T, d, _handle(stream, dev)), w)
+    _used(stream, x, weight, residual, y, residual_out)
     return y, residual_out, q, s
 
 
@@ -174,6 +183,7 @@ class KvCache:
         self.k, self.v, self.k_scale, self.v_scale, self.pages = k, v, k_scale, v_scale, pages
         self._s = _CacheStruct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, self.heads, self.page, self.dim)
         self._ref = ctypes.byref(self._s)
+        self.tensors = (k, v, k_scale, v_scale)
 
     @classmethod
     def empty(cls, pages: int, heads: int, dim: int, page: int = 64, device="cuda"):
@@ -246,6 +256,7 @@ def rope_append(cache: KvCache, table, lens, q, k, v, turns=None, cu=None, pos=N
     check(lib().vkb_rope_append(cache._ref, table.data_ptr(), table.shape[1], lens.data_ptr(), _p(cu), B, T, dt,
                                 _p(q), ldq, _p(q_out), ldo, hq, k.data_ptr(), ldk, v.data_ptr(), ldv, _p(pos),
                                 _p(turns), rot, lay, mscale, _handle(stream, dev)), w)
+    _used(stream, table, lens, q, k, v, turns, cu, pos, q_out, *cache.tensors)
     return q_out
 
 
@@ -264,6 +275,7 @@ def kv_read(cache: KvCache, table, seq, pos, dtype=torch.float16, stream=None):
     v = _made(k, stream)
     check(lib().vkb_kv_read(cache._ref, table.data_ptr(), table.shape[1], table.shape[0], seq.data_ptr(), pos.data_ptr(), n,
                             _DT[dtype], k.data_ptr(), v.data_ptr(), _handle(stream, dev)), w)
+    _used(stream, table, seq, pos, *cache.tensors)
     return k, v
 
 
@@ -305,6 +317,7 @@ def attention(cache: KvCache, table, lens, q, cu=None, scale: float | None = Non
     check(lib().vkb_attention(cache._ref, table.data_ptr(), table.shape[1], lens.data_ptr(), _p(cu), B, T, _DT[q.dtype],
                               q.data_ptr(), ldq, out.data_ptr(), ldo, hq, cache.dim ** -0.5 if scale is None else scale,
                               window, work.data_ptr(), work.numel() * work.element_size(), _handle(stream, dev)), w)
+    _used(stream, table, lens, q, cu, out, work, *cache.tensors)
     return out
 
 
@@ -333,4 +346,5 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, toke
         _array(w, "token", token, B, torch.int32, dev)
     check(lib().vkb_sample(dt, logits.data_ptr(), logits.stride(0) if B > 1 else V, B, V, _p(temperature), _p(top_k), _p(top_p),
                            _p(min_p), u.data_ptr(), token.data_ptr(), prob.data_ptr(), _handle(stream, dev)), w)
+    _used(stream, logits, u, temperature, top_k, top_p, min_p, token, prob)
     return token, prob
