@@ -251,6 +251,9 @@ def test_bad_indices_are_reported(cuda):
     many = torch.zeros((2 * 40, 4, 64), device="cuda").half()
     vkb.attention(cache, bad, ln, many, cu=offsets([40, 40]), work=work)
     assert vkb.device_status() == 16
+    wide = torch.zeros((2 * 40, 64, 64), device="cuda").half()
+    vkb.attention(cache, bad, ln, wide, cu=offsets([40, 40]), work=work)
+    assert vkb.device_status() == 16
     k, v = vkb.kv_read(cache, table, torch.tensor([0, 5], dtype=torch.int32, device="cuda"), torch.tensor([99, 0], dtype=torch.int32, device="cuda"))
     assert float(k.abs().max()) == 0.0 and vkb.device_status() == 16
     out = vkb.attention(cache, table, ln, q, work=work)      # and the workspace is ready for the next call
@@ -329,6 +332,67 @@ def test_attention(cuda, case, x_dt):
     assert torch.equal(first, check_attention(cache, table, lens, news, q, window))      # the order of arrival does not matter
 
 
+PROMPTS = [   # enough query rows for the prompt kernel at every dimension: lens, news, kv heads, q heads, dim, page, window
+    ([300], [300], 2, 16, 128, 64, 0),
+    ([520, 0, 129, 64], [190, 0, 129, 1], 2, 24, 128, 16, 0),
+    ([700, 33], [260, 33], 1, 20, 96, 128, 100),
+    ([257, 400], [257, 90], 4, 16, 112, 32, 0),
+    ([200], [200], 3, 39, 48, 16, 65),
+    ([1030, 5, 64], [500, 5, 64], 1, 16, 64, 64, 0),
+    ([600], [129], 1, 37, 192, 32, 0),
+    ([700], [290], 2, 16, 256, 128, 300),
+    ([1500, 1], [130, 1], 2, 64, 240, 16, 1),
+    ([150, 100], [170, 100], 2, 32, 128, 64, 0),      # more new tokens than the sequence is long
+]
+
+
+@pytest.mark.parametrize("case", PROMPTS, ids=[str(i) for i in range(len(PROMPTS))])
+@pytest.mark.parametrize("x_dt", ["float16", "bfloat16"])
+def test_attention_prompts(cuda, case, x_dt):
+    import torch
+    lens, news, heads, hq, dim, page, window = case
+    assert sum(news) * hq > 4096
+    cache, table, _ = make_cache(lens, heads, dim, page, seed=dim + hq)
+    q = (torch.randn((sum(news), hq + 2, dim), generator=gen(7), device="cuda") * 1.5).to(dt(x_dt))[:, 1:hq + 1]
+    work = vkb.attention_workspace(cache)
+    first = check_attention(cache, table, lens, news, q, window, work=work)
+    assert torch.equal(first, check_attention(cache, table, lens, news, q, window, work=work))
+
+
+def test_attention_prompt_scales_and_nan(cuda):
+    """test_attention_scales' pages and a NaN row, with enough q heads for the prompt kernel."""
+    import torch
+    lens, news = [400, 150], [120, 150]
+    cache, table, ln = make_cache(lens, 2, 64, 16, seed=3)
+    for page_at, k, v in ((3, 1.0, 0.0), (5, 0.0, 1.0), (7, 1.0, 1e4), (8, 1.0, 1e-5), (11, 30.0, 1.0)):
+        pg = table[0, page_at].long()
+        cache.k_scale[pg] *= k
+        cache.v_scale[pg] *= v
+        if k == 0.0:
+            cache.k[pg] = 128
+        if v == 0.0:
+            cache.v[pg] = 128
+    cache.v_scale[table[1, 0].long()] = 0.0
+    cache.v[table[1, 0].long()] = 128
+    for mag in (1e-3, 1.0, 30.0):
+        q = (torch.randn((270, 32, 64), generator=gen(2), device="cuda") * mag).to(torch.bfloat16)
+        check_attention(cache, table, lens, news, q)
+        check_attention(cache, table, lens, news, q.half(), scale=0.03)
+    q = q.half() * 0.02
+    cu = offsets(news)
+    want = vkb.attention(cache, table, ln, q, cu=cu)
+    q[130, 17, 5] = float("nan")
+    out = vkb.attention(cache, table, ln, q, cu=cu)
+    keep = torch.ones(out.shape[:2], dtype=torch.bool, device="cuda")
+    keep[130, 17] = False
+    assert bool(torch.isnan(out[130, 17]).all()) and bool(torch.isfinite(out[keep]).all())
+    assert float((out[keep].double() - want[keep].double()).abs().max()) <= 2.0 ** -9 * float(want.abs().max())
+    cache.v_scale.zero_()
+    cache.v.fill_(128)
+    q[130, 17, 5] = 0.0
+    assert float(check_attention(cache, table, lens, news, q).abs().max()) == 0.0
+
+
 @pytest.mark.parametrize("n_new", [1, 3, 64])
 def test_attention_scales(cuda, n_new):
     """Pages whose scales are zero, tiny or huge beside one another, sharp and flat scores, q of large and small magnitude."""
@@ -397,7 +461,7 @@ def test_attention_offsets_past_32_bits(cuda):
     cache = vkb.KvCache(k, v, s[0].contiguous(), s[1].contiguous())
     table = torch.tensor([[pages - 1, pages - 4], [pages - 2, pages - 6]], dtype=torch.int32, device="cuda")
     lens = [200, 131]
-    for news in ([1, 1], [4, 3], [90, 60]):
+    for news in ([1, 1], [4, 3], [90, 60], [200, 131]):
         T = sum(news)
         q = torch.randn((T, 16, dim), generator=g, device="cuda").half()
         kn = torch.randn((T, heads, dim), generator=g, device="cuda").half()

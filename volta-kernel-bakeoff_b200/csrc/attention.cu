@@ -69,21 +69,26 @@ static int launch_prompt(const vkb_kv_cache_t* c, const AttnArgs& a, int dev, cu
 
 template <typename T>
 static int attn_dispatch(const vkb_kv_cache_t* c, const AttnArgs& a, int dev, cudaStream_t st) {
-    // Query rows per sequence and kv head, on average: the smallest tile of the token kernel that holds them; the prompt
-    // kernel where they are more than its largest.
+    // Query rows per sequence and kv head, on average: the token kernel with the smallest tile that holds them. More rows
+    // than its largest tile go to the prompt kernel, whose tile reads the keys once for 256 rows (128 at dimension 256), unless
+    // the call is so small that the token kernel's many small items keep the SMs busier. Measured (32 q heads on 8,
+    // dimension 128, B200): one sequence of 8192 keys, 64 rows 40 us against 48, 256 rows 81 against 108, 512 rows 130
+    // against 98; 16 sequences of 1500 keys, 64 rows 83 against 66; 16 q heads on 2, dimension 256: one of 8192 keys, 256 rows 48
+    // against 214, 16 of 1500 keys, 128 rows 72 against 101, 384 rows 174 against 107.
     const long long rows = ((long long)a.T + a.B - 1) / a.B * a.G;
+    const bool few = (long long)a.T * a.G * a.heads <= (c->dim > 128 ? 4096 : 2560);
     switch (attn_dt(c->dim)) {
         case 64:
-            return rows <= 8    ? launch_token<64, 1, T>(c, a, dev, st)
-                   : rows <= 16 ? launch_token<64, 2, T>(c, a, dev, st)
-                   : rows <= 32 ? launch_token<64, 4, T>(c, a, dev, st) : launch_prompt<64, T>(c, a, dev, st);
+            if (rows <= 8) return launch_token<64, 1, T>(c, a, dev, st);
+            if (rows <= 16) return launch_token<64, 2, T>(c, a, dev, st);
+            return rows <= 32 || few ? launch_token<64, 4, T>(c, a, dev, st) : launch_prompt<64, T>(c, a, dev, st);
         case 128:
-            return rows <= 8    ? launch_token<128, 1, T>(c, a, dev, st)
-                   : rows <= 16 ? launch_token<128, 2, T>(c, a, dev, st)
-                   : rows <= 32 ? launch_token<128, 4, T>(c, a, dev, st) : launch_prompt<128, T>(c, a, dev, st);
+            if (rows <= 8) return launch_token<128, 1, T>(c, a, dev, st);
+            if (rows <= 16) return launch_token<128, 2, T>(c, a, dev, st);
+            return rows <= 32 || few ? launch_token<128, 4, T>(c, a, dev, st) : launch_prompt<128, T>(c, a, dev, st);
         default:
-            return rows <= 8    ? launch_token<256, 1, T>(c, a, dev, st)
-                   : rows <= 16 ? launch_token<256, 2, T>(c, a, dev, st) : launch_prompt<256, T>(c, a, dev, st);
+            if (rows <= 8) return launch_token<256, 1, T>(c, a, dev, st);
+            return rows <= 16 || few ? launch_token<256, 2, T>(c, a, dev, st) : launch_prompt<256, T>(c, a, dev, st);
     }
 }
 
