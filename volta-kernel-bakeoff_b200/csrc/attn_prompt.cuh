@@ -226,10 +226,11 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
     bool ok = true;
     int jj = 0;          // key tiles so far, over all items of the run
 
-    // Registers: 512 threads are launched with 128 each; the warpgroups take 64, 128 and 2 x 160 (NT = 1: 64, 2 x 128 and
-    // 192), 512 x 128 in all. The split stands at the head of each role, where the compiler counts from it.
+    // Registers: 512 threads are launched with 128 each (65536); the warpgroups take 56, 104 and 2 x 176 (65536), with NT = 1
+    // 56, 2 x 128 and 192. The split stands at the head of each role, where the compiler counts from it. (160 for the softmax
+    // and 128 to convert: 1.24 ms for the chunk of 4096 behind 12288 tokens, against 1.21.)
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 0) {
         // ===================== MMA issuer =====================
         const uint32_t id_s = umma_idesc_f16(PR_KT), id_o = umma_idesc_f16(DT) | (1u << 16);   // V': MN-major B
@@ -320,6 +321,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
         }
         }
     } else if (warp >= 16 - C::ND / 32) {
+        if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
         // ===================== convert codes =====================
         constexpr int CPR = DT / 16, NB = PR_KT * CPR / C::ND;   // 16-code chunks per row; per thread and tile
         constexpr int RSTEP = C::ND / CPR;                        // rows between a thread's chunks (a multiple of 16)
@@ -405,7 +407,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
             jj += max(n, 0);
         }
     } else {
-        if constexpr (NT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
+        if constexpr (NT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
         else asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
         // ===================== softmax: a row per thread =====================
         const int t = (warp - 4) >> 2, q4 = warp & 3, r = 128 * t + 32 * q4 + lane;   // row tile, lane quarter, row
