@@ -18,8 +18,10 @@
 //   warps 4-7     softmax of row tile 0, a row per thread (tensor memory lanes are rows)
 //   warps 8-11    softmax of row tile 1 (NT = 2: dimensions up to 128); convert codes (NT = 1: dimension 256, where O
 //                 takes half of tensor memory)
-//   warps 12-15   convert codes: global loads of 16 codes, a tile ahead in registers, to 128-byte swizzled fp16 tiles
+//   warps 12-15   convert codes: global loads of 16 codes, two tiles ahead in registers, to 128-byte swizzled fp16 tiles
 //                 (K: K-major B operand; V: the same bytes are the MN-major B operand of P V)
+// Measured on a B200 (32 q heads on 8, dimension 128): 4096 tokens behind 12288 take 1.21 ms, 795 TFLOP/s on the causal
+// pairs; the tensor pipe is busy for 35 % of it, the exponentials for a third: bound by the softmax warps' issue.
 #pragma once
 
 #include "attn_token.cuh"

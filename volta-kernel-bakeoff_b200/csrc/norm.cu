@@ -4,7 +4,9 @@
 //
 // HBM-bound: every input element is read once and every output written once. A row belongs to one group of threads:
 // thread t holds the vectors of eight t, t + threads, ... in registers between the reduction and the output, so the
-// row is not read again; rows of up to 512 elements take one warp each (no block-wide barrier), four rows to a block.
+// row is not read again; rows of up to 512 elements, and wider ones where there are thousands, take one warp each (no
+// block-wide barrier), four rows to a block. Measured on a B200, bf16 with residual in and out: 8191 x 2560 in 34 us, 4.9
+// TB/s, with the Q8 copy 42 us.
 // Rows that are not made of aligned vectors of eight (odd widths, odd strides) go element by element and read their
 // inputs a second time (from L1 / L2) instead of holding them.
 #include "step.cuh"
