@@ -1,0 +1,68 @@
+"""Edge cases of the decode-step operators on the GPU. Helpers and the derivation of the tolerances: test_step_gpu.py."""
+import pytest
+
+import vkb
+from test_step_gpu import check_attention, dt, gen, make_cache
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- V scales that grow within a segment ------------------------------------------------------------------------------
+
+def quiet_pages(cache, table, b, first, last, scale):
+    """The pages of tokens [first, last) of sequence b get V scale `scale` (0: codes of zero too)."""
+    for pg in table[b, first // cache.page:-(-last // cache.page)].long().tolist():
+        cache.v_scale[pg] = scale
+        if scale == 0.0:
+            cache.v[pg] = 128
+
+
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64), (128, 128), (256, 32), (256, 128)])
+@pytest.mark.parametrize("quiet", [64, 128, 576])
+@pytest.mark.parametrize("scale", [0.01, 0.06, 1.0, 50.0])
+def test_first_keys_without_values(cuda, dim, page, quiet, scale):
+    """Keys whose V scale is 0 keep their weight, also where they fill the first tiles that a block reads."""
+    import torch
+    lens, news = [quiet + 700, quiet + 90], [200, 80]
+    cache, table, _ = make_cache(lens, 1, dim, page, seed=dim + page)
+    cache.v_scale[:] = scale
+    for b in range(2):
+        quiet_pages(cache, table, b, 0, quiet, 0.0)
+    q = (torch.randn((280, 16, dim), generator=gen(quiet), device="cuda") * 1.5).half()
+    check_attention(cache, table, lens, news, q)                                      # many rows
+    check_attention(cache, table, lens, [1, 1], q[:2])                                # a token each
+
+
+def come_and_go(dim, low, high):
+    """A sequence of 6000 keys with stretches of 512 of V scale `low` and of `high` in turn."""
+    cache, table, ln = make_cache([6000], 1, dim, 64, seed=dim)
+    cache.v_scale[:] = high
+    for at in range(0, 6000, 1024):
+        quiet_pages(cache, table, 0, at, min(6000, at + 512), low)
+    return cache, table, ln
+
+
+@pytest.mark.parametrize("low,high,x_dt", [(0.0, 0.1, "float16"), (0.0, 1.0, "bfloat16"), (1e-30, 1.0, "float16"), (1e-9, 1.0, "bfloat16")])
+@pytest.mark.parametrize("dim", [128, 256])
+def test_values_that_come_and_go(cuda, low, high, x_dt, dim):
+    """Blocks that take parts of an item start in stretches of either kind."""
+    import torch
+    cache, table, _ = come_and_go(dim, low, high)
+    q = (torch.randn((300, 16, dim), generator=gen(dim), device="cuda") * 1.5).to(dt(x_dt))
+    check_attention(cache, table, [6000], [300], q)
+    check_attention(cache, table, [6000], [1], q[:1])
+
+
+@pytest.mark.parametrize("low", [0.0, 1e-9, 0.2])
+@pytest.mark.parametrize("new", [1, 300])
+def test_outputs_follow_the_v_scales(cuda, low, new):
+    """V scales times a power of two: the outputs times that power, exactly (bf16 holds them all)."""
+    import torch
+    cache, table, ln = come_and_go(128, low, 30.0)
+    q = (torch.randn((new, 16, 128), generator=gen(new), device="cuda") * 1.5).to(torch.bfloat16)
+    cu = torch.tensor([0, new], dtype=torch.int32, device="cuda")
+    want = vkb.attention(cache, table, ln, q, cu=cu)
+    for k in (-5, 3, 60):
+        cache.v_scale *= 2.0 ** k
+        assert torch.equal(vkb.attention(cache, table, ln, q, cu=cu), want * 2.0 ** k), k
+        cache.v_scale *= 2.0 ** -k

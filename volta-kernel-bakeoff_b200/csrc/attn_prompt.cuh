@@ -2,19 +2,21 @@
 //
 // An item is a tile of NT x 128 query rows; per 64 keys S = Q K'^T and O += P V' are tcgen05.mma with fp32
 // accumulators in tensor memory, K' and V' the codes as exact fp16 integers in shared memory, converted once for all
-// rows of the tile. The scales never touch the codes: with x_j = s_j ks_j scale log2(e) + log2(vs_j / vs0),
-//   p'_j = 2^(x_j - M + 8),   O' = sum_j p'_j c'_j,   l = sum_j p'_j (vs0 / vs_j),   o = vs0 O' / l,
+// rows of the tile. The scales never touch the codes: with x_j = s_j ks_j scale log2(e) + log2(vs_j / V),
+//   p'_j = 2^(x_j - M + 8),   O' = sum_j p'_j c'_j,   l = sum_j p'_j (V / vs_j),   o = V O' / l,
 // so a group of 16 keys (a page or part of one) costs one multiply-add per score and one multiply per group. p' is
 // rounded once, to fp16, for the product; l sums it in fp32. M follows the running maximum of x lazily, so that O' is
-// rescaled only when a p' might leave fp16's range. vs0: the largest V scale of the segment's first keys; scales
-// below 2^-30 of the largest seen so far count as that.
+// rescaled only when a p' might leave fp16's range. V is the power of two at or below the largest V scale seen so far (so
+// that it seldom moves: O' is rescaled then too); scales below 2^-30 of that largest count as 2^-30 of it. V follows upwards
+// because M would have to stand in for it otherwise: behind first keys of scale 0 M jumped past what 2^(M - M') holds, and
+// their part of l was lost.
 //
 // 16 warps, one block per SM (its run of units: attn_common.cuh):
 //   warp 0        issues the MMAs. S has two buffers of 64 columns per row tile, and P takes its S's place: S(j + 1) is
 //                 issued before P(j) is there, so that the softmax goes from one tile to the next without waiting for
 //                 an MMA (with one buffer of 128 keys the two waited for each other: 7700 cycles per 128 keys, the
 //                 softmax busy for 3800 of them)
-//   warp 1        makes the scale tables {ks scale log2(e), log2(vs / vs0), vs0 / vs} of the groups of 16 keys
+//   warp 1        makes the scale tables {ks scale log2(e), log2(vs / V), V / vs, V} of the groups of 16 keys
 //   warps 4-7     softmax of row tile 0, a row per thread (tensor memory lanes are rows)
 //   warps 8-11    softmax of row tile 1 (NT = 2: dimensions up to 128); convert codes (NT = 1: dimension 256, where O
 //                 takes half of tensor memory)
@@ -46,7 +48,7 @@ template <int DT> struct PrCfg {
     static constexpr int q_off = 0;
     static constexpr int k_off = NT * QTILE;
     static constexpr int v_off = k_off + NS * TILE;
-    static constexpr int sc_off = v_off + NS * TILE;              // [PR_SCT][4] {kf, lv, iv, vs0}
+    static constexpr int sc_off = v_off + NS * TILE;              // [PR_SCT][4] {kf, lv, iv, V}
     static constexpr int row_off = sc_off + PR_SCT * 4 * 16;      // [ROWS] factor of q
     static constexpr int bar_off = row_off + ROWS * 4;
     static constexpr int NBAR = 1 + 4 * NS + 4 + 4 + 4 + 4;
@@ -292,7 +294,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
         int nb = 0;   // batches so far
         while (ok && attn_next<C::ROWS, PR_KT, PR_OV>(a, run, &g)) {
             const int n = g.t1 - g.t0;
-            float vs0 = 0.f, cmax = 0.f;   // reference and largest V scale of the segment
+            float cmax = 7.888609e-31f;   // 2^-100, then the segment's largest V scale
             int next = pr_page(a, g, g.t0, lane);
             for (int j0 = 0; j0 < n && ok; j0 += 8, ++nb) {
                 int id = next;
@@ -305,7 +307,6 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
                 }
                 float most = fmaxf(vs, __shfl_xor_sync(0xffffffffu, vs, 1));
                 most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-                if (j0 == 0) vs0 = fmaxf(__shfl_sync(0xffffffffu, most, 0), 7.888609e-31f);   // 2^-100
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) {   // largest of this tile and the ones before it
                     const float v = __shfl_up_sync(0xffffffffu, most, o);
@@ -313,10 +314,10 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
                 }
                 most = fmaxf(most, cmax);
                 cmax = __shfl_sync(0xffffffffu, most, 31);
-                const float ref = fmaxf(most, vs0) * 9.313226e-10f;   // 2^-30
-                const float lv = log2f(__fdiv_rn(fmaxf(vs, ref), vs0));
+                const float V = __uint_as_float(__float_as_uint(most) & 0x7f800000u);   // its power of two
+                const float lv = log2f(__fdiv_rn(fmaxf(vs, most * 9.313226e-10f), V));    // 2^-30
                 if (nb >= 2) ok = __all_sync(0xffffffffu, wait_parity_sleep(&sc_empty[nb & 1], ((nb >> 1) - 1) & 1));
-                sct[(nb & 1) * 32 + lane] = make_float4(ks * a.scale_log2, lv, exp2f(-lv), vs0);
+                sct[(nb & 1) * 32 + lane] = make_float4(ks * a.scale_log2, lv, exp2f(-lv), V);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sc_full[nb & 1]);
             }
@@ -469,7 +470,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
             const float qinv = bf && n > 0 ? __fdiv_rn(1.f, rowf[r]) : 1.f;
             const int all_hi = __reduce_min_sync(0xffffffffu, khi);   // keys [all_lo, all_hi): all the warp's rows see them
             const int all_lo = __reduce_max_sync(0xffffffffu, klo);
-            float M = -INFINITY, vs0 = 0.f;
+            float M = -INFINITY, V = 0.f;
             uint64_t l2 = 0;   // the sum of p, two halves
             for (int j = 0; j < n; ++j) {
                 const int J = jj + j, buf = 2 * t + (J & 1), key0 = (g.t0 + j) * PR_KT;
@@ -495,19 +496,19 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
                         }
                     }
                 };
-                vs0 = sc[0].w;
+                const float v1 = sc[0].w;
                 read();
                 // ---- p' against the M of the tiles before this one, and its sum. Where eight p' of a row add up to more than
                 // 2^15 (so that one of them might pass fp16's 65504), M is moved up to the maximum and the tile is done
-                // again: the first tile that a row sees, and few others, so that the maximum of the scores is not taken
-                // ahead of everything else ----
+                // again: the first tile that a row sees, the tiles where V moves, and few others, so that the maximum of the
+                // scores is not taken ahead of everything else ----
                 uint32_t pk[16], pk2[16];
                 uint64_t sum = 0;
                 float mb = M == -INFINITY ? 0.f : M - PR_BIAS, top = 0.f;
                 pr_exp(s, pk, sc, qinv, mb, sum, top);
                 pr_exp(s2, pk2, sc + 2, qinv, mb, sum, top);
                 const bool unset = M == -INFINITY && klo < key0 + PR_KT && khi > key0;   // the row's first keys
-                if (__any_sync(0xffffffffu, unset || top > 32768.f)) {
+                if (__any_sync(0xffffffffu, unset || top > 32768.f || v1 != V)) {
                     read();   // again, so that the scores need not stay in registers meanwhile
                     const float mx = pr_max(s2, sc + 2, qinv, pr_max(s, sc, qinv, -INFINITY));
                     const float mn = fmaxf(M, mx), al = M == -INFINITY ? 0.f : ex2(M - mn);
@@ -517,15 +518,17 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
                         if (ok) ok = __all_sync(0xffffffffu, wait_parity_sleep(&o_full[2 * t + ((J - 1) & 1)], ((J - 1) >> 1) & 1));
                         tc_fence_after();
                         const uint32_t to = tl + C::o_col + t * DT;
+                        const float of = al * __fdiv_rn(V, v1);   // O' in units of the new V
 #pragma unroll 1
                         for (int c = 0; c < DT / 32; ++c) {
                             tmem_ld32(to + 32 * c, s);
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) * al);
+                            for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) * of);
                             tmem_st32(to + 32 * c, s);
                         }
                         read();
                     }
+                    V = v1;
                     sum = 0;
                     mb = M == -INFINITY ? 0.f : M - PR_BIAS;
                     pr_exp(s, pk, sc, qinv, mb, sum, top);
@@ -550,7 +553,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
             const uint32_t to = tl + C::o_col + t * DT;
             constexpr int PITCH = DT + 2;
             float* part = a.part + attn_slot(g, blockIdx.x) * C::ROWS * PITCH;
-            const float inv = g.whole ? (l == 0.f ? 0.f : __fdiv_rn(vs0, l)) : vs0;
+            const float inv = g.whole ? (l == 0.f ? 0.f : __fdiv_rn(V, l)) : V;
             const bool live = M > -INFINITY || M != M || l != 0.f;   // rows that saw a key
             T* out = attn_out<T>(a, g, rr);
             if (r < g.rows && !g.whole) *reinterpret_cast<float2*>(part + C::ROWS * DT + 2 * r) = make_float2(M, l);
