@@ -146,7 +146,8 @@ def rope_turns(rot: int, base: float = 10000.0, scaling: str | None = None, fact
     elif scaling == "parts":
         def pair(turns):   # the (fractional) pair that turns this many times in `original` positions
             return rot * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))
-        lo, hi = max(0, math.floor(pair(beta_fast))), min(n - 1, math.ceil(pair(beta_slow)))
+        # the ramp may end past the last pair, which then keeps a share of its frequency
+        lo, hi = max(0, math.floor(pair(beta_fast))), min(rot - 1, math.ceil(pair(beta_slow)))
         for i in range(n):
             r = min(1.0, max(0.0, (i - lo) / max(1e-3, hi - lo)))
             freq[i] *= (1 - r) + r / factor
