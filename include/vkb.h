@@ -157,7 +157,8 @@ int vkb_rms_norm(int dt, const void* x, long long ldx, const void* res, void* re
  * rows are cu[b] .. cu[b + 1] - 1 of the call's T rows, its last cu[b + 1] - cu[b] tokens (cu null: one row per
  * sequence, T == B). A sequence of length 0 is an idle one: nothing is written for it and its attention output is
  * zero. Rows outside every sequence's span are not written. Lengths, offsets and pages outside their arrays are skipped
- * (a sequence whose length or offsets are out of range is left out) and raise bit 16 of vkb_device_status. */
+ * (a sequence whose length or offsets are out of range is left out; the tokens of a page that does not exist are not
+ * written, read as zeros and take no weight in attention) and raise bit 16 of vkb_device_status. */
 typedef struct vkb_kv_cache {
     void* k;
     void* v;

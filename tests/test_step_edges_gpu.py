@@ -1,8 +1,10 @@
 """Edge cases of the decode-step operators on the GPU. Helpers and the derivation of the tolerances: test_step_gpu.py."""
+import math
+
 import pytest
 
 import vkb
-from test_step_gpu import check_attention, dt, gen, make_cache
+from test_step_gpu import U, check_attention, dt, gen, make_cache, offsets, values
 
 pytestmark = pytest.mark.gpu
 
@@ -66,3 +68,58 @@ def test_outputs_follow_the_v_scales(cuda, low, new):
         cache.v_scale *= 2.0 ** k
         assert torch.equal(vkb.attention(cache, table, ln, q, cu=cu), want * 2.0 ** k), k
         cache.v_scale *= 2.0 ** -k
+
+
+# ---- pages that do not exist ------------------------------------------------------------------------------------------
+
+def masked_ref(cache, table, lens, news, q, gone, window=0):
+    """attention_ref() without the keys of the pages `gone` [(sequence, page of it)]: their weight set to zero."""
+    import torch
+    fixed = table.clone()
+    for b, i in gone:
+        fixed[b, i] = int(table[b, 0]) if int(table[b, 0]) >= 0 else 0
+    o, tol = torch.zeros(q.shape, dtype=torch.float64, device="cuda"), torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+    at, grp = 0, q.shape[1] // cache.heads
+    for b, (n, m) in enumerate(zip(lens, news)):
+        k, v = values(cache, fixed, b, n)
+        pos, j = torch.arange(n - m, n, device="cuda")[:, None], torch.arange(n, device="cuda")[None]
+        seen = (j <= pos) & (j > pos - window if window else j >= 0)
+        for x, i in gone:
+            if x == b:
+                seen = seen & ~((j >= i * cache.page) & (j < (i + 1) * cache.page))
+        for h in range(q.shape[1]):
+            x, kh, vh = q[at:at + m, h].double(), k[:, h // grp], v[:, h // grp]
+            s = (x @ kh.T * cache.dim ** -0.5).masked_fill(~seen, -math.inf)
+            p = torch.softmax(s, -1).nan_to_num(0.0)
+            o[at:at + m, h] = p @ vh
+            terms = (x.abs() @ kh.abs().T * cache.dim ** -0.5).masked_fill(~seen, 0.0).amax(-1, keepdim=True)
+            tol[at:at + m, h] = (p @ vh.abs()) * (2.0 ** -11 + 2 * terms * 2 * cache.dim * 2.0 ** -24 + 2.0 ** -21 * 8)
+        at += m
+    u = U[str(q.dtype).split(".")[1]]
+    return o, tol * (1 + u) + o.abs() * u * 1.01 + 1e-6
+
+
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 32), (128, 64), (256, 128), (80, 16)])
+@pytest.mark.parametrize("new", [1, 4, 150])
+@pytest.mark.parametrize("bad", [-1, 1 << 20, None])
+def test_keys_of_pages_outside_the_cache_are_left_out(cuda, dim, page, new, bad):
+    """They take no weight (a page index that does not exist: bit 16), whatever page 0 holds."""
+    import torch
+    lens, news = [520, 300], [new, new]
+    cache, table, ln = make_cache(lens, 1, dim, page, seed=page)
+    unused = sorted(set(range(cache.pages)) - set(table[table >= 0].tolist()))[0]
+    table[table == 0] = unused                      # page 0: no sequence's, loud
+    cache.k_scale[0], cache.v_scale[0] = 3.0, 1000.0
+    gone = [(0, 0), (0, 2), (1, 1)]
+    table2 = table.clone()
+    for b, i in gone:
+        table2[b, i] = cache.pages if bad is None else bad
+    q = (torch.randn((2 * new, 16, dim), generator=gen(new), device="cuda")).half()
+    out = vkb.attention(cache, table2, ln, q, cu=offsets(news))
+    torch.cuda.synchronize()
+    assert vkb.device_status() == 16
+    o, tol = masked_ref(cache, table, lens, news, q, gone)
+    assert not bool(((out.double() - o).abs() > tol).any()), float((out.double() - o).abs().max())
+    table2[1] = -1                                   # a sequence without any page: zeros
+    out = vkb.attention(cache, table2, ln, q, cu=offsets(news))
+    assert float(out[new:].abs().max()) == 0.0 and bool(torch.isfinite(out).all()) and vkb.device_status() == 16

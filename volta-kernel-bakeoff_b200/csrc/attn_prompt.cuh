@@ -317,7 +317,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
                 const float V = __uint_as_float(__float_as_uint(most) & 0x7f800000u);   // its power of two
                 const float lv = log2f(__fdiv_rn(fmaxf(vs, most * 9.313226e-10f), V));    // 2^-30
                 if (nb >= 2) ok = __all_sync(0xffffffffu, wait_parity_sleep(&sc_empty[nb & 1], ((nb >> 1) - 1) & 1));
-                sct[(nb & 1) * 32 + lane] = make_float4(ks * a.scale_log2, lv, exp2f(-lv), V);
+                // keys of no page: weight 0, whatever their scores
+                sct[(nb & 1) * 32 + lane] = id >= 0 ? make_float4(ks * a.scale_log2, lv, exp2f(-lv), V)
+                                                    : make_float4(0.f, -INFINITY, 0.f, V);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sc_full[nb & 1]);
             }

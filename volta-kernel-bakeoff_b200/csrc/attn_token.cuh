@@ -32,6 +32,9 @@ constexpr int TK_OV = 16;                            // an item's own cost in un
 constexpr int TK_STREAMS = 4;                        // streaming warps
 constexpr float TK_P_BIAS = 8.f;                     // p' is kept times 2^8
 
+// The {K, V} scales of keys whose page does not exist.
+static __device__ const float tk_no_page[2] = {-INFINITY, 0.f};
+
 // DT: head dimension rounded up to 64, 128 or 256. NQ: tiles of 8 query rows per item.
 template <int DT, int NQ> struct TkCfg {
     static constexpr int ROWS = 8 * NQ;
@@ -198,9 +201,11 @@ attn_token_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
                     have = p0;
                     ids = p0 + lane < a.table_ld ? row[p0 + lane] : -1;
                 }
-                // lane i < np: piece i's page; a page index outside the cache reads page 0 and raises a status bit
+                // lane i < np: piece i's page. A page index outside the cache raises a status bit; its boxes come from page
+                // 0, and its scales from a pair that tells the computing warps to leave the keys out
                 int id = __shfl_sync(0xffffffffu, ids, (p0 - have + min(lane, np - 1)) & 31);
-                if (id < 0 || id >= a.pages) {
+                const bool none = id < 0 || id >= a.pages;
+                if (none) {
                     if (lane < np) raise_status(DEV_ERR_BAD_INDEX);
                     id = 0;
                 }
@@ -217,8 +222,10 @@ attn_token_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
                         tma_load_2d(d + C::TILE + hf * AT_KT * 128, &tv, hf * 128, y, &full[st]);
                     }
                     const uint32_t sd = smem_u32(scales + st * 8 + 2 * lane);
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sd), "l"(a.ks + ph) : "memory");
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sd + 4), "l"(a.vs + ph) : "memory");
+                    const float* ks = none ? tk_no_page : a.ks + ph;
+                    const float* vs = none ? tk_no_page + 1 : a.vs + ph;
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sd), "l"(ks) : "memory");
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sd + 4), "l"(vs) : "memory");
                 }
                 asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[st])) : "memory");
                 __syncwarp();
@@ -301,9 +308,9 @@ attn_token_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             if (!ok) continue;   // the wait gave up (status bit): the walk goes on so that every arrival is made
             const uint32_t kt = smem_u32(sm + st * C::STAGE), vt = kt + C::TILE;
             const int key0 = (g.t0 + i) * AT_KT + wk;
-            if (key0 < g.len) {
-                const int piece = a.page_log2 >= 6 ? 0 : wk >> a.page_log2;
-                const float2 sc = *reinterpret_cast<const float2*>(scales + st * 8 + 2 * piece);
+            const int piece = a.page_log2 >= 6 ? 0 : wk >> a.page_log2;   // one page's keys, or none that exist
+            const float2 sc = *reinterpret_cast<const float2*>(scales + st * 8 + 2 * piece);
+            if (key0 < g.len && sc.x != -INFINITY) {
                 float s[NQ][4];
 #pragma unroll
                 for (int nq = 0; nq < NQ; ++nq)
