@@ -123,3 +123,18 @@ def test_keys_of_pages_outside_the_cache_are_left_out(cuda, dim, page, new, bad)
     table2[1] = -1                                   # a sequence without any page: zeros
     out = vkb.attention(cache, table2, ln, q, cu=offsets(news))
     assert float(out[new:].abs().max()) == 0.0 and bool(torch.isfinite(out).all()) and vkb.device_status() == 16
+
+
+@pytest.mark.parametrize("new", [1, 5, 150])
+@pytest.mark.parametrize("page", [16, 64, 128])
+def test_pages_behind_the_window_may_be_given_back(cuda, new, page):
+    """Pages that no row of the call sees are not looked at: a caller may take them out of the table."""
+    import torch
+    lens, news, window = [1003, 700], [new, new], 77
+    cache, table, ln = make_cache(lens, 2, 128, page)
+    q = torch.randn((2 * new, 32, 128), generator=gen(new), device="cuda").half()
+    want = vkb.attention(cache, table, ln, q, cu=offsets(news), window=window)
+    for b, n in enumerate(lens):
+        table[b, :max(0, n - new - window + 1) // page] = -1
+    out = vkb.attention(cache, table, ln, q, cu=offsets(news), window=window)
+    assert vkb.device_status() == 0 and torch.equal(out, want)

@@ -214,6 +214,12 @@ template <int ROWS, int KT, int OV> __device__ __forceinline__ bool attn_next(co
 // Where a part of block c goes: slot 1 for the item that starts in the block, 0 for one that started earlier.
 __device__ __forceinline__ long long attn_slot(const AttnSeg& g, int c) { return 2ll * c + (g.c0 == c ? 1 : 0); }
 
+// The first key that any row of the segment sees. Pages that end before it are not looked at: where a window has passed
+// them the caller may have given them to another sequence.
+__device__ __forceinline__ int attn_first_key(const AttnArgs& a, const AttnSeg& g) {
+    return a.window > 0 ? max(0, g.pos0 + g.r0 / a.G - a.window + 1) : 0;
+}
+
 // Output row of row r of a segment.
 template <typename T> __device__ __forceinline__ T* attn_out(const AttnArgs& a, const AttnSeg& g, int r) {
     const int t = (g.r0 + r) / a.G, hq = g.h * a.G + (g.r0 + r) - t * a.G;

@@ -169,10 +169,15 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Eight tiles from t on, a lane per group of 16 keys: the group's page, -1 where there is none.
-__device__ __forceinline__ int pr_page(const AttnArgs& a, const AttnSeg& g, int t, int lane) {
+// Eight tiles from t on, a lane per group of 16 keys: whether any row may see the group (first: attn_first_key), and its
+// page, -1 where none does.
+__device__ __forceinline__ bool pr_seen(const AttnSeg& g, int first, int t, int lane) {
     const int key = (t + (lane >> 2)) * PR_KT + 16 * (lane & 3);
-    return t + (lane >> 2) < g.t1 && key < g.len ? a.table[(long long)g.b * a.table_ld + (key >> a.page_log2)] : -1;
+    return t + (lane >> 2) < g.t1 && key < g.len && key + 16 > first;
+}
+__device__ __forceinline__ int pr_page(const AttnArgs& a, const AttnSeg& g, int first, int t, int lane) {
+    const int key = (t + (lane >> 2)) * PR_KT + 16 * (lane & 3);
+    return pr_seen(g, first, t, lane) ? a.table[(long long)g.b * a.table_ld + (key >> a.page_log2)] : -1;
 }
 
 template <int DT, typename T>
@@ -293,12 +298,12 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
         // ===================== scale tables =====================
         int nb = 0;   // batches so far
         while (ok && attn_next<C::ROWS, PR_KT, PR_OV>(a, run, &g)) {
-            const int n = g.t1 - g.t0;
+            const int n = g.t1 - g.t0, first = attn_first_key(a, g);
             float cmax = 7.888609e-31f;   // 2^-100, then the segment's largest V scale
-            int next = pr_page(a, g, g.t0, lane);
+            int next = pr_page(a, g, first, g.t0, lane);
             for (int j0 = 0; j0 < n && ok; j0 += 8, ++nb) {
                 int id = next;
-                next = pr_page(a, g, g.t0 + j0 + 8, lane);
+                next = pr_page(a, g, first, g.t0 + j0 + 8, lane);
                 if (id >= a.pages) id = -1;
                 float ks = 0.f, vs = 0.f;
                 if (id >= 0) {
@@ -355,14 +360,14 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
         };
         struct Tile { uint4 k[NB], v[NB]; };   // a tile's codes on their way to shared memory
         while (ok && attn_next<C::ROWS, PR_KT, PR_OV>(a, run, &g)) {
-            const int n = g.t1 - g.t0;
+            const int n = g.t1 - g.t0, first = attn_first_key(a, g);
             // eight tiles' groups, a lane each: where their codes start, -1 where there are none
             long long base = -1;
-            int next = pr_page(a, g, g.t0, lane);
+            int next = pr_page(a, g, first, g.t0, lane);
             auto enter = [&](int t) {
                 int id = next;
-                next = pr_page(a, g, t + 8, lane);
-                if (id >= a.pages || (id < 0 && t + (lane >> 2) < g.t1 && (t + (lane >> 2)) * PR_KT + 16 * (lane & 3) < g.len)) {
+                next = pr_page(a, g, first, t + 8, lane);
+                if (id >= a.pages || (id < 0 && pr_seen(g, first, t, lane))) {
                     raise_status(DEV_ERR_BAD_INDEX);
                     id = -1;
                 }

@@ -189,6 +189,7 @@ attn_token_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         while (ok && attn_next<C::ROWS, AT_KT, TK_OV>(a, run, &g)) {
             const int32_t* row = a.table + (long long)g.b * a.table_ld;
             int have = -1, ids = -1;   // this lane's page id of pages [have, have + 32)
+            const int first = attn_first_key(a, g) >> a.page_log2;   // pages before it: behind every row's window
             for (int t = g.t0; t < g.t1; ++t, ++it) {
                 if ((it & (TK_STREAMS - 1)) != stream) continue;
                 const int st = it % C::NS;
@@ -201,12 +202,13 @@ attn_token_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
                     have = p0;
                     ids = p0 + lane < a.table_ld ? row[p0 + lane] : -1;
                 }
-                // lane i < np: piece i's page. A page index outside the cache raises a status bit; its boxes come from page
-                // 0, and its scales from a pair that tells the computing warps to leave the keys out
+                // lane i < np: piece i's page. For one that no row sees, or a page index outside the cache (which raises a
+                // status bit), the boxes come from page 0, and the scales from a pair that tells the computing warps to
+                // leave the keys out
                 int id = __shfl_sync(0xffffffffu, ids, (p0 - have + min(lane, np - 1)) & 31);
-                const bool none = id < 0 || id >= a.pages;
+                const bool unseen = p0 + lane < first, none = unseen || id < 0 || id >= a.pages;
                 if (none) {
-                    if (lane < np) raise_status(DEV_ERR_BAD_INDEX);
+                    if (lane < np && !unseen) raise_status(DEV_ERR_BAD_INDEX);
                     id = 0;
                 }
                 uint8_t* dst = sm + st * C::STAGE;
