@@ -1,5 +1,6 @@
 """Edge cases of the decode-step operators' boundary that need no GPU."""
 import math
+import os
 
 import pytest
 
@@ -25,3 +26,14 @@ def test_parts_by_how_often_a_pair_turns(rot, base, original, factor):
             assert abs(g / f - 1) < 1e-12, i
     last = original * plain[-1] / (2 * math.pi)
     assert (parts[-1] / plain[-1] > 1 / factor + 1e-3) == (last > 1.1)      # divided in full only where it turns less than once
+
+
+def test_no_non_coherent_loads_of_what_an_earlier_grid_writes():
+    """These kernels are launched while the grid before may still be writing their inputs. Loads through the non-coherent path
+    are for data that nobody writes while the kernel is resident; griddepcontrol.wait promises nothing for them."""
+    root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "volta-kernel-bakeoff_b200", "csrc")
+    for name in ("step.cuh", "norm.cu", "kv_cache.cu", "attention.cu", "attn_common.cuh", "attn_token.cuh", "attn_prompt.cuh", "sample.cu"):
+        with open(os.path.join(root, name)) as f:
+            text = f.read()
+        for word in ("__ldg", ".nc.", "__restrict__"):
+            assert word not in text, (name, word)

@@ -20,8 +20,8 @@
 //   warps 4-7     softmax of row tile 0, a row per thread (tensor memory lanes are rows)
 //   warps 8-11    softmax of row tile 1 (NT = 2: dimensions up to 128); convert codes (NT = 1: dimension 256, where O
 //                 takes half of tensor memory)
-//   warps 12-15   convert codes: global loads of 16 codes, two tiles ahead in registers, to 128-byte swizzled fp16 tiles
-//                 (K: K-major B operand; V: the same bytes are the MN-major B operand of P V)
+//   warps 12-15   convert codes: global loads of 16 codes (past L1: each is read once), two tiles ahead in registers, to
+//                 128-byte swizzled fp16 tiles (K: K-major B operand; V: the same bytes are the MN-major B operand of P V)
 // Measured on a B200 (32 q heads on 8, dimension 128): 4096 tokens behind 12288 take 1.21 ms, 795 TFLOP/s on the causal
 // pairs; the tensor pipe is busy for 35 % of it, the exponentials for a third: bound by the softmax warps' issue.
 #pragma once
@@ -182,8 +182,8 @@ __device__ __forceinline__ int pr_page(const AttnArgs& a, const AttnSeg& g, int 
 
 template <int DT, typename T>
 __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid_constant__ AttnArgs a,
-                                                                    const uint8_t* __restrict__ kc,
-                                                                    const uint8_t* __restrict__ vc) {
+                                                                    const uint8_t* kc,
+                                                                    const uint8_t* vc) {
     using C = PrCfg<DT>;
     constexpr int NT = C::NT, NS = C::NS;
     extern __shared__ uint8_t smem_raw[];
@@ -307,8 +307,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
                 if (id >= a.pages) id = -1;
                 float ks = 0.f, vs = 0.f;
                 if (id >= 0) {
-                    ks = __ldg(a.ks + (long long)id * a.heads + g.h);
-                    vs = __ldg(a.vs + (long long)id * a.heads + g.h);
+                    ks = __ldcg(a.ks + (long long)id * a.heads + g.h);
+                    vs = __ldcg(a.vs + (long long)id * a.heads + g.h);
                 }
                 float most = fmaxf(vs, __shfl_xor_sync(0xffffffffu, vs, 1));
                 most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
@@ -384,8 +384,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
                     const long long p = __shfl_sync(0xffffffffu, base, 4 * (j & 7) + ((r0 + e * RSTEP) >> 4));
                     x.k[e] = x.v[e] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
                     if (p >= 0 && e * RSTEP < left && col) {
-                        x.k[e] = __ldg(reinterpret_cast<const uint4*>(kc + p + toff));
-                        x.v[e] = __ldg(reinterpret_cast<const uint4*>(vc + p + toff));
+                        x.k[e] = __ldcg(reinterpret_cast<const uint4*>(kc + p + toff));
+                        x.v[e] = __ldcg(reinterpret_cast<const uint4*>(vc + p + toff));
                     }
                 }
             };
