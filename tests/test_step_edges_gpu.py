@@ -4,7 +4,7 @@ import math
 import pytest
 
 import vkb
-from test_step_gpu import U, check_attention, dt, gen, make_cache, offsets, values
+from test_step_gpu import U, check_attention, dt, gen, make_cache, offsets, turned, values
 
 pytestmark = pytest.mark.gpu
 
@@ -138,3 +138,30 @@ def test_pages_behind_the_window_may_be_given_back(cuda, new, page):
         table[b, :max(0, n - new - window + 1) // page] = -1
     out = vkb.attention(cache, table, ln, q, cu=offsets(news), window=window)
     assert vkb.device_status() == 0 and torch.equal(out, want)
+
+
+# ---- rows of no sequence ----------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("with_pos", [False, True])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_rope_append_leaves_rows_of_no_sequence(cuda, with_pos, layout):
+    import torch
+    g = gen(1)
+    cache, table, _ = make_cache([20, 30, 9], 1, 64, 16)
+    ln = torch.tensor([20, 1000, 9], dtype=torch.int32, device="cuda")     # the second is longer than its table
+    cu = torch.tensor([1, 4, 6, 9], dtype=torch.int32, device="cuda")      # rows 0 and 9.. are nobody's
+    q, k, v = (torch.randn((12, h, 64), generator=g, device="cuda") for h in (2, 1, 1))
+    turns, _ = vkb.rope_turns(64)
+    pos = torch.arange(100, 112, dtype=torch.int32, device="cuda") if with_pos else None
+    out = torch.full_like(q, 7.0)
+    vkb.rope_append(cache, table, ln, q, k, v, turns=turns, cu=cu, pos=pos, layout=layout, q_out=out)
+    assert vkb.device_status() == 16
+    same = q.clone()
+    vkb.rope_append(cache, table, ln, same, k, v, turns=turns, cu=cu, pos=pos, layout=layout, q_out=same)
+    assert vkb.device_status() == 16
+    mine = [1, 2, 3, 6, 7, 8]
+    rest = [i for i in range(12) if i not in mine]
+    assert bool((out[rest] == 7.0).all()) and torch.equal(same[rest], q[rest]) and torch.equal(same[mine], out[mine])
+    at = pos[mine].tolist() if with_pos else [17, 18, 19, 6, 7, 8]
+    want = turned(q[mine].double(), at, turns, layout)
+    assert float((out[mine].double() - want).abs().max()) <= 2.0 ** -20 * float(q.abs().max())

@@ -151,25 +151,21 @@ template <int DT> __global__ void __launch_bounds__(AP_THREADS) rope_append_kern
     const int dv = a.dim >> 3;
     if ((int)blockIdx.x >= nkv) {   // ---- one token's q heads ----
         const int t = blockIdx.x - nkv;
-        long long pos;
-        if (a.pos) pos = a.pos[t];
-        else {   // the sequence of token t: the number of sequences that end at or before it
-            int b = t;
-            if (a.cu) {
-                int n = 0;
-                for (int i = tid; i < a.B; i += AP_THREADS) n += a.cu[i + 1] <= t;
-                n = __reduce_add_sync(0xffffffffu, n);
-                if (lane == 0) sh[warp] = n;
-                __syncthreads();
-                b = 0;
+        int b = t;   // the sequence of token t: the number of sequences that end at or before it
+        if (a.cu) {
+            int n = 0;
+            for (int i = tid; i < a.B; i += AP_THREADS) n += a.cu[i + 1] <= t;
+            n = __reduce_add_sync(0xffffffffu, n);
+            if (lane == 0) sh[warp] = n;
+            __syncthreads();
+            b = 0;
 #pragma unroll
-                for (int w = 0; w < AP_THREADS / 32; ++w) b += sh[w];
-            }
-            if (b >= a.B) return;   // rows past the last sequence
-            const SeqSpan s = seq_span(a, b);
-            if (t < s.q0 || t >= s.q0 + s.n) return;
-            pos = (long long)s.len - s.n + (t - s.q0);
+            for (int w = 0; w < AP_THREADS / 32; ++w) b += sh[w];
         }
+        if (b >= a.B) return;   // rows past the last sequence
+        const SeqSpan s = seq_span(a, b);
+        if (t < s.q0 || t >= s.q0 + s.n) return;   // rows of no sequence, or of one that is left out
+        const long long pos = a.pos ? a.pos[t] : (long long)s.len - s.n + (t - s.q0);
         float2* cs = reinterpret_cast<float2*>(ap_smem);
         for (int i = tid; i < a.half_rot; i += AP_THREADS) cs[i] = rope_cs(a, pos, i);
         __syncthreads();
