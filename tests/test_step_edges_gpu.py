@@ -165,3 +165,16 @@ def test_rope_append_leaves_rows_of_no_sequence(cuda, with_pos, layout):
     at = pos[mine].tolist() if with_pos else [17, 18, 19, 6, 7, 8]
     want = turned(q[mine].double(), at, turns, layout)
     assert float((out[mine].double() - want).abs().max()) <= 2.0 ** -20 * float(q.abs().max())
+
+
+# ---- windows and counts near 2^31 -------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("window", [(1 << 31) - 1, (1 << 31) - 20])
+@pytest.mark.parametrize("lens,news,hq", [([3], [30], 1), ([100, 30], [170, 90], 32)])
+def test_window_wider_than_any_sequence(cuda, window, lens, news, hq):
+    """With more new tokens than the sequence is long, the first rows lie before position 0."""
+    import torch
+    cache, table, _ = make_cache(lens, 1, 64, 16)
+    q = torch.randn((sum(news), hq, 64), generator=gen(2), device="cuda").half()
+    out = check_attention(cache, table, lens, news, q, window)
+    assert torch.equal(out, check_attention(cache, table, lens, news, q, 0))

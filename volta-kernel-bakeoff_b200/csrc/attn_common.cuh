@@ -50,11 +50,13 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnArgs& a, int b) {
     }
     return s;
 }
+// The window's first key for a row at position p (at most 0: all). Rows before position 0 see no key; they count as position
+// 0 here, so that no window, however wide, wraps around.
+__device__ __forceinline__ int attn_window(const AttnArgs& a, int p) { return a.window > 0 ? max(p, 0) - a.window + 1 : 0; }
 // The key tiles [t0, t1) of rows [r0, r1) of a sequence (t1 <= t0: no row sees a key).
 template <int KT> __device__ __forceinline__ void attn_tiles(const AttnArgs& a, const AttnSeq& s, int r0, int r1, int* t0, int* t1) {
     const int first = s.len - s.n + r0 / a.G, last = s.len - s.n + (r1 - 1) / a.G;   // token positions
-    const int lo = a.window > 0 ? max(0, first - a.window + 1) : 0;
-    *t0 = lo / KT;
+    *t0 = max(0, attn_window(a, first)) / KT;
     *t1 = last >= 0 ? (last + KT) / KT : 0;
     if (*t1 < *t0) *t1 = *t0;
 }
@@ -217,7 +219,7 @@ __device__ __forceinline__ long long attn_slot(const AttnSeg& g, int c) { return
 // The first key that any row of the segment sees. Pages that end before it are not looked at: where a window has passed
 // them the caller may have given them to another sequence.
 __device__ __forceinline__ int attn_first_key(const AttnArgs& a, const AttnSeg& g) {
-    return a.window > 0 ? max(0, g.pos0 + g.r0 / a.G - a.window + 1) : 0;
+    return max(0, attn_window(a, g.pos0 + g.r0 / a.G));
 }
 
 // Output row of row r of a segment.

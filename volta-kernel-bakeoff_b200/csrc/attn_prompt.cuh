@@ -473,7 +473,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
                 if (lane == 0) mbar_arrive(q_full);
             }
             const int rr = min(r, g.rows - 1), pos = g.pos0 + (g.r0 + rr) / a.G;
-            const int khi = r < g.rows ? pos + 1 : 0, klo = a.window > 0 ? pos - a.window + 1 : 0;
+            const int khi = r < g.rows ? pos + 1 : 0, klo = attn_window(a, pos);
             const float qinv = bf && n > 0 ? __fdiv_rn(1.f, rowf[r]) : 1.f;
             const int all_hi = __reduce_min_sync(0xffffffffu, khi);   // keys [all_lo, all_hi): all the warp's rows see them
             const int all_lo = __reduce_max_sync(0xffffffffu, klo);

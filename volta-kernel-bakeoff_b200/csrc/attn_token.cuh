@@ -285,11 +285,11 @@ attn_token_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
                 const int r = 8 * nq + 2 * qc + e, rr = min(r, g.rows - 1);
                 const int p = g.pos0 + (g.r0 + rr) / a.G;
                 khi[nq][e] = r < g.rows ? p + 1 : 0;
-                klo[nq][e] = a.window > 0 ? p - a.window + 1 : 0;
+                klo[nq][e] = attn_window(a, p);
             }
         // keys that every row of the tile sees: no mask needed (rows past the tile's compute what is not written)
         const int all_hi = g.pos0 + g.r0 / a.G + 1;
-        const int all_lo = a.window > 0 ? g.pos0 + (g.r0 + g.rows - 1) / a.G - a.window + 1 : 0;
+        const int all_lo = attn_window(a, g.pos0 + (g.r0 + g.rows - 1) / a.G);
 
         float o[NQ][KS][4];   // O^T: dimension 16 j + 2 gr (and + 1: elements 2, 3), queries 2 qc, 2 qc + 1
         float M[NQ][2], l[NQ][2], V = 7.888609e-31f, vinv = 1.2676506e30f;   // 2^-100
