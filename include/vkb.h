@@ -153,12 +153,12 @@ int vkb_rms_norm(int dt, const void* x, long long ldx, const void* res, void* re
  * page: 16, 32, 64 or 128 tokens; dim: a multiple of 16 up to 256. A sequence's token p is in slot p % page of page
  * table[b][p / page] (int32 [B][table_ld]); pages may come in any order and may be shared, except that a page being
  * appended to belongs to one sequence.
- * The calls below take lens [B]: each sequence's length including the call's new tokens, and cu [B + 1]: sequence b's
- * rows are cu[b] .. cu[b + 1] - 1 of the call's T rows, its last cu[b + 1] - cu[b] tokens (cu null: one row per
- * sequence, T == B). A sequence of length 0 is an idle one: nothing is written for it and its attention output is
- * zero. Rows outside every sequence's span are not written. Lengths, offsets and pages outside their arrays are skipped
- * (a sequence whose length or offsets are out of range is left out; the tokens of a page that does not exist are not
- * written, read as zeros and take no weight in attention) and raise bit 16 of vkb_device_status. */
+ * The calls below take lens [B]: each sequence's length including the call's new tokens (up to 2^31 - 4096), and
+ * cu [B + 1]: sequence b's rows are cu[b] .. cu[b + 1] - 1 of the call's T rows, its last cu[b + 1] - cu[b] tokens (cu
+ * null: one row per sequence, T == B). A sequence of length 0 is an idle one: nothing is written for it and its attention
+ * output is zero. Rows outside every sequence's span are not written. Lengths, offsets and pages outside their arrays are
+ * skipped (a sequence whose length or offsets are out of range is left out; the tokens of a page that does not exist are
+ * not written, read as zeros and take no weight in attention) and raise bit 16 of vkb_device_status. */
 typedef struct vkb_kv_cache {
     void* k;
     void* v;

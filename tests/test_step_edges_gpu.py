@@ -178,3 +178,32 @@ def test_window_wider_than_any_sequence(cuda, window, lens, news, hq):
     q = torch.randn((sum(news), hq, 64), generator=gen(2), device="cuda").half()
     out = check_attention(cache, table, lens, news, q, window)
     assert torch.equal(out, check_attention(cache, table, lens, news, q, 0))
+
+
+def test_lengths_near_2_31(cuda):
+    """A table of 2^31 tokens, all of them in a few pages: the longest length works, a longer one is left out."""
+    import torch
+    page, longest = 128, (1 << 31) - 4096
+    cache, _, _ = make_cache([3 * page], 1, 64, page, spare=0)
+    table = torch.full((1, (1 << 31) // page), 0, dtype=torch.int32, device="cuda")
+    at = (longest - 1) // page
+    table[0, at - 1], table[0, at] = 1, 2
+    g = gen(5)
+    q, k, v = (torch.randn((2, h, 64), generator=g, device="cuda").half() for h in (4, 1, 1))
+    cu, ln = offsets([2]), torch.tensor([longest], dtype=torch.int32, device="cuda")
+    held = cache.k[:2].clone()
+    vkb.rope_append(cache, table, ln, None, k, v, cu=cu)
+    seq, pos = torch.zeros(2, dtype=torch.int32, device="cuda"), torch.tensor([longest - 2, longest - 1], dtype=torch.int32, device="cuda")
+    kk, _ = vkb.kv_read(cache, table, seq, pos)
+    assert float((kk.double() - k.double()).abs().max()) <= float(cache.k_scale[2, 0])
+    out = vkb.attention(cache, table, ln, q, cu=cu, window=200)
+    short = torch.tensor([[1, 2]], dtype=torch.int32, device="cuda")       # the same two pages as a short sequence
+    want = vkb.attention(cache, short, torch.tensor([2 * page], dtype=torch.int32, device="cuda"), q, cu=cu, window=200)
+    assert vkb.device_status() == 0 and torch.equal(out, want) and torch.equal(cache.k[:2], held)
+    snap = cache.k.clone()
+    for n in (longest + 1, (1 << 31) - 1):
+        ln.fill_(n)
+        vkb.rope_append(cache, table, ln, None, k, v, cu=cu)
+        assert vkb.device_status() == 16 and torch.equal(cache.k, snap)
+        vkb.attention(cache, table, ln, q, cu=cu, window=200)
+        assert vkb.device_status() == 16

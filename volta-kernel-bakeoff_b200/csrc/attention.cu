@@ -117,7 +117,7 @@ extern "C" int vkb_attention(const vkb_kv_cache_t* c, const int32_t* table, int 
     if (!q || !out || ldq < row || ldo < row) return VKB_EINVAL;
     if (!work || !aligned_to(work, 16) || work_bytes < vkb_attention_work_bytes(c->dim)) return VKB_EINVAL;
     if (!aligned_to(q, 16) || !aligned_to(out, 16) || ldq % 8 || ldo % 8) return VKB_EUNSUPPORTED;
-    if ((long long)T * (q_heads / c->heads) > 0x7fffffffll) return VKB_EUNSUPPORTED;
+    if ((long long)T * (q_heads / c->heads) > MAX_POSITIONS) return VKB_EUNSUPPORTED;
     int dev = 0;
     if (int r = current_device(&dev)) return r;
     if ((size_t)device_info(dev).sm_count * sizeof(unsigned) > ATTN_CNT_BYTES) return VKB_EUNSUPPORTED;
@@ -131,7 +131,7 @@ extern "C" int vkb_attention(const vkb_kv_cache_t* c, const int32_t* table, int 
     a.scale_log2 = scale * 1.4426950408889634f;
     a.B = B; a.T = T; a.heads = c->heads; a.G = q_heads / c->heads; a.dim = c->dim; a.pages = c->pages;
     a.page_log2 = c->page == 16 ? 4 : c->page == 32 ? 5 : c->page == 64 ? 6 : 7;
-    a.table_ld = table_ld; a.window = window;
+    a.table_ld = table_ld; a.window = window; a.max_len = max_length(table_ld, c->page);
     cudaStream_t st = (cudaStream_t)stream;
     return dt == VKB_DT_F16 ? attn_dispatch<__half>(c, a, dev, st) : attn_dispatch<__nv_bfloat16>(c, a, dev, st);
 }

@@ -31,7 +31,7 @@ struct AttnArgs {
     unsigned* cnt;        // [grid] arrivals of the item that starts in this block; zero between calls
     long long ldq, ldo;
     float scale_log2;     // scale * log2(e)
-    int B, T, heads, G, dim, pages, page_log2, table_ld, window;
+    int B, T, heads, G, dim, pages, page_log2, table_ld, window, max_len;
 };
 
 struct AttnSeq {
@@ -44,7 +44,7 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnArgs& a, int b) {
     s.len = a.lens[b];
     s.q0 = a.cu ? a.cu[b] : b;
     s.n = a.cu ? a.cu[b + 1] - s.q0 : 1;
-    if (s.len < 0 || s.n < 0 || s.q0 < 0 || s.q0 > a.T - s.n || s.len > ((long long)a.table_ld << a.page_log2)) {
+    if (s.len < 0 || s.n < 0 || s.q0 < 0 || s.q0 > a.T - s.n || s.len > a.max_len) {
         raise_status(DEV_ERR_BAD_INDEX);
         s.len = s.n = 0;
     }

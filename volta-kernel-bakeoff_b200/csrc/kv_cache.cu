@@ -36,6 +36,7 @@ struct AppendArgs {
     const void* kv[2];
     long long ldq, ldqo, ldkv[2];
     int pages, heads, page, dim, table_ld, B, T, hq, half_rot, layout, items;
+    int max_len;                         // of a sequence
     int cs_max, cs_tokens, val_tokens;   // shared memory: cosines in all, of how many tokens; values of how many tokens
     float mscale;
 };
@@ -115,7 +116,7 @@ __device__ __forceinline__ SeqSpan seq_span(const AppendArgs& a, int b) {
     s.len = a.lens[b];
     s.q0 = a.cu ? a.cu[b] : b;
     s.n = a.cu ? a.cu[b + 1] - s.q0 : 1;
-    if (s.len < 0 || s.n < 0 || s.q0 < 0 || s.q0 > a.T - s.n || s.len > (long long)a.table_ld * a.page) {
+    if (s.len < 0 || s.n < 0 || s.q0 < 0 || s.q0 > a.T - s.n || s.len > a.max_len) {
         raise_status(DEV_ERR_BAD_INDEX);
         s.n = 0;
     }
@@ -440,6 +441,7 @@ extern "C" int vkb_rope_append(const vkb_kv_cache_t* c, const int32_t* table, in
     a.pages = c->pages; a.heads = c->heads; a.page = c->page; a.dim = c->dim; a.table_ld = table_ld;
     a.B = B; a.T = T; a.hq = q_heads; a.half_rot = rot / 2; a.layout = layout; a.items = (int)items;
     a.mscale = mscale;
+    a.max_len = max_length(table_ld, c->page);
     // Shared memory of a block: cosines and sines of 1024 pairs (or one token's), values of a page's tokens up to 40 KB (five
     // blocks per SM); single tokens take what one needs.
     const int pairs = rot / 2 > 0 ? rot / 2 : 1, value = 4 * (c->dim + 4);

@@ -16,6 +16,13 @@ namespace vkb {
 
 enum : unsigned { DEV_ERR_BAD_INDEX = 16u };   // a length, offset or page index outside its array: that part skipped
 
+// Positions and row counts stay 4096 below 2^31, so that the end of a tile, a page or a batch of tiles is still an int.
+constexpr long long MAX_POSITIONS = 0x7ffff000ll;
+inline int max_length(int table_ld, int page) {   // the longest sequence that a table row holds
+    const long long n = (long long)table_ld * page;
+    return (int)(n < MAX_POSITIONS ? n : MAX_POSITIONS);
+}
+
 template <int DT> struct Elem;
 template <> struct Elem<VKB_DT_F16> {
     using T = __half;
