@@ -158,7 +158,8 @@ int vkb_rms_norm(int dt, const void* x, long long ldx, const void* res, void* re
  * null: one row per sequence, T == B). A sequence of length 0 is an idle one: nothing is written for it and its attention
  * output is zero. Rows outside every sequence's span are not written. Lengths, offsets and pages outside their arrays are
  * skipped (a sequence whose length or offsets are out of range is left out; the tokens of a page that does not exist are
- * not written, read as zeros and take no weight in attention) and raise bit 16 of vkb_device_status. */
+ * not written, read as zeros and take no weight in attention; offsets that decrease from one sequence to the next leave
+ * the whole call of vkb_attention out) and raise bit 16 of vkb_device_status. */
 typedef struct vkb_kv_cache {
     void* k;
     void* v;

@@ -207,3 +207,30 @@ def test_lengths_near_2_31(cuda):
         assert vkb.device_status() == 16 and torch.equal(cache.k, snap)
         vkb.attention(cache, table, ln, q, cu=cu, window=200)
         assert vkb.device_status() == 16
+
+
+@pytest.mark.parametrize("T,hq,tile", [(16, 32, 8), (16, 256, 32), (64, 512, 256)])     # the last: the prompt kernel
+def test_overlapping_spans_of_more_units_than_the_division_holds(cuda, T, hq, tile):
+    """Offsets 0, T, 0, T, ..: every second sequence has all rows, and their units in all pass 2^31. The call is left out."""
+    import torch
+    B, page = 1024, 128
+    cache, _, _ = make_cache([page], 8, 64, page, spare=0)
+    table = torch.zeros((B, 65536), dtype=torch.int32, device="cuda")
+    ln = torch.full((B,), 65536 * page // 2, dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, T] * (B // 2) + [0], dtype=torch.int32, device="cuda")
+    q, out = torch.zeros((T, hq, 64), device="cuda").half(), torch.full((T, hq, 64), 7.0, device="cuda").half()
+    assert B // 2 * 8 * -(-T * hq // 8 // tile) * (int(ln[0]) // 64 + 16) >= (1 << 31) - 1
+    vkb.attention(cache, table, ln, q, cu=cu, out=out)
+    assert vkb.device_status() == 16 and bool((out == 7.0).all())
+    check_attention(cache, table[:2, :1].contiguous(), [100, 128], [1, 1], q[:2])        # the next call is right
+
+
+def test_offsets_that_decrease(cuda):
+    import torch
+    cache, table, ln = make_cache([40, 40, 40], 1, 64, 16)
+    for hq in (4, 128):
+        q = torch.randn((40, hq, 64), generator=gen(3), device="cuda").half()
+        out = torch.full_like(q, 7.0)
+        vkb.attention(cache, table, ln, q, cu=torch.tensor([0, 30, 10, 40], dtype=torch.int32, device="cuda"), out=out)
+        assert vkb.device_status() == 16 and bool((out == 7.0).all())
+        check_attention(cache, table, [40, 40, 40], [10, 5, 25], q)

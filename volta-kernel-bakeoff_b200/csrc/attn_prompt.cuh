@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
     if (warp == 0) tmem_alloc<1>(tmem_slot, 512);
     tc_fence_before();
     pdl_wait();
-    AttnRun run = attn_run<C::ROWS, PR_KT, PR_OV, PR_THREADS>(a, run_sh);   // its barriers publish the above
+    AttnRun run = attn_run<C::ROWS, PR_KT, PR_OV, PR_THREADS>(a, run_sh, join_sh + 2);   // its barriers publish the above
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     AttnSeg g;

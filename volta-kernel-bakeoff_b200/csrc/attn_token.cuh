@@ -176,7 +176,7 @@ attn_token_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         prefetch_tmap(&tv);
     }
     pdl_wait();
-    AttnRun run = attn_run<C::ROWS, AT_KT, TK_OV, C::THREADS>(a, run_sh);   // its barriers also publish the mbarriers
+    AttnRun run = attn_run<C::ROWS, AT_KT, TK_OV, C::THREADS>(a, run_sh, join_sh + 1);   // its barriers also publish the mbarriers
     AttnSeg g;
 
     if (warp >= C::WARPS) {
