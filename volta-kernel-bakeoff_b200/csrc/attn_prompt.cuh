@@ -51,7 +51,7 @@ template <int DT> struct PrCfg {
     static constexpr int sc_off = v_off + NS * TILE;              // [PR_SCT][4] {kf, lv, iv, V}
     static constexpr int row_off = sc_off + PR_SCT * 4 * 16;      // [ROWS] factor of q
     static constexpr int bar_off = row_off + ROWS * 4;
-    static constexpr int NBAR = 1 + 4 * NS + 4 + 4 + 4 + 4;
+    static constexpr int NBAR = 1 + 4 * NS + 4 + 4 + 4 + 4 + 1;
     static constexpr int run_off = bar_off + NBAR * 8;
     static constexpr int BYTES = run_off + 4 * (PR_THREADS / 32 + 2) + 16 + 1024;
     static constexpr int o_col = 256;                             // O of row tile t at o_col + t DT; its S buffers at
@@ -200,6 +200,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
     uint64_t* o_full = p_full + 4;        // [2 t + tile parity] O of the row tile updated
     uint64_t* sc_full = o_full + 4;       // [2] eight tiles' scale tables written
     uint64_t* sc_empty = sc_full + 2;     // [2] and read (NT * 4 warps)
+    uint64_t* done = sc_empty + 2;        // every MMA of the block done
     unsigned* run_sh = reinterpret_cast<unsigned*>(sm + C::run_off);
     volatile int* join_sh = reinterpret_cast<volatile int*>(run_sh + PR_THREADS / 32 + 2);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(run_sh + PR_THREADS / 32 + 2) + 1;
@@ -208,6 +209,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
     pdl_trigger();
     if (threadIdx.x == 0) {
         mbar_init(q_full, NT * 4);
+        mbar_init(done, 1);
         for (int i = 0; i < NS; ++i) {
             mbar_init(&k_full[i], C::ND / 32);
             mbar_init(&k_empty[i], 1);
@@ -294,6 +296,10 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
             }
             jj += n;
         }
+        // drain: every MMA is done before tensor memory is freed, also where a wait gave up
+        if (elect_one()) umma_commit(done);
+        __syncwarp();
+        wait_parity_sleep(done, 0, DEV_ERR_DRAIN_TIMEOUT);
         } else if (warp == 1) {
         // ===================== scale tables =====================
         int nb = 0;   // batches so far
@@ -484,7 +490,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
                 if (ok && (j & 7) == 0)
                     ok = __all_sync(0xffffffffu, wait_parity_sleep(&sc_full[nb & 1], (nb >> 1) & 1));
                 if (ok) ok = __all_sync(0xffffffffu, wait_parity_sleep(&s_full[buf], (J >> 1) & 1));
-                if (!ok) continue;   // the wait gave up (status bit): the walk goes on so that every arrival is made
+                if (!ok) continue;   // the wait gave up (status bit): the walk goes on to the items' joins, whose barriers and
+                                     // counts the other warps and blocks need (the pipeline's waits give up one after another)
                 tc_fence_after();
                 const float4* sc = sct + (nb & 1) * 32 + (j & 7) * 4;
                 const uint32_t ts = tl + 64 * buf;
@@ -589,7 +596,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) attn_prompt_kernel(const __grid
             if (!g.whole) attn_join<DT, C::ROWS, T>(a, g, stid, nsm, join_sh, bar);
         }
     }
-    // The softmax warps have waited for the last O update, and so for every MMA, before tensor memory is freed
+    // The issuing warp has waited for every MMA, the softmax warps for their own loads, before tensor memory is freed
     tc_fence_before();
     __syncthreads();
     tc_fence_after();

@@ -307,7 +307,8 @@ attn_token_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         for (int i = (grp - it) & (C::GROUPS - 1); i < n; i += C::GROUPS) {
             const int u = it + i, st = u % C::NS;
             if (ok) ok = __all_sync(0xffffffffu, wait_parity(&full[st], (u / C::NS) & 1));
-            if (!ok) continue;   // the wait gave up (status bit): the walk goes on so that every arrival is made
+            if (!ok) continue;   // the wait gave up (status bit): the walk goes on to the items' joins, whose barriers and counts
+                                 // the other warps and blocks need (the streaming warps' waits give up too)
             const uint32_t kt = smem_u32(sm + st * C::STAGE), vt = kt + C::TILE;
             const int key0 = (g.t0 + i) * AT_KT + wk;
             const int piece = a.page_log2 >= 6 ? 0 : wk >> a.page_log2;   // one page's keys, or none that exist
