@@ -37,3 +37,13 @@ def test_no_non_coherent_loads_of_what_an_earlier_grid_writes():
             text = f.read()
         for word in ("__ldg", ".nc.", "__restrict__"):
             assert word not in text, (name, word)
+
+
+def test_arguments_that_are_no_tensors_are_refused():
+    """None or a list in the place of a tensor is a refusal like any other, not an AttributeError."""
+    import torch
+    x = torch.zeros(2, 64)
+    for name, call in {"x": lambda: vkb.rms_norm(None, x[0]), "logits": lambda: vkb.sample([0.0], x[0]),
+                       "cache": lambda: vkb.attention(None, x, x, x), "k": lambda: vkb.KvCache(None, x, x, x)}.items():
+        with pytest.raises(vkb.VkbError, match=name):
+            call()

@@ -234,3 +234,34 @@ def test_offsets_that_decrease(cuda):
         vkb.attention(cache, table, ln, q, cu=torch.tensor([0, 30, 10, 40], dtype=torch.int32, device="cuda"), out=out)
         assert vkb.device_status() == 16 and bool((out == 7.0).all())
         check_attention(cache, table, [40, 40, 40], [10, 5, 25], q)
+
+
+# ---- refusals ---------------------------------------------------------------------------------------------------------
+
+def test_arguments_that_are_no_tensors_are_refused(cuda):
+    """None where an argument must be given, plain numbers in the place of arrays, windows that a C int does not hold."""
+    import torch
+    cache, table, ln = make_cache([20, 20], 1, 64, 16)
+    x, w = torch.zeros((2, 64), device="cuda"), torch.ones(64, device="cuda")
+    q, u = torch.zeros((2, 1, 64), device="cuda").half(), torch.zeros(2, device="cuda")
+    i32 = torch.zeros(2, dtype=torch.int32, device="cuda")
+    for name, call in (
+            ("weight", lambda: vkb.rms_norm(x, None)), ("residual", lambda: vkb.rms_norm(x, w, 1.0)), ("y", lambda: vkb.rms_norm(x, w, y=0)),
+            ("residual_out", lambda: vkb.rms_norm(x, w, x, residual_out=0)),
+            ("k", lambda: vkb.rope_append(cache, table, ln, q, None, q)), ("v", lambda: vkb.rope_append(cache, table, ln, q, q, None)),
+            ("q", lambda: vkb.rope_append(cache, table, ln, 1, q, q)), ("table", lambda: vkb.rope_append(cache, None, ln, q, q, q)),
+            ("lens", lambda: vkb.rope_append(cache, table, None, q, q, q)), ("turns", lambda: vkb.rope_append(cache, table, ln, q, q, q, turns=64)),
+            ("turns", lambda: vkb.rope_append(cache, table, ln, q, q, q, turns=torch.tensor(5, device="cuda"))),
+            ("pos", lambda: vkb.rope_append(cache, table, ln, q, q, q, pos=3)), ("q_out", lambda: vkb.rope_append(cache, table, ln, q, q, q, q_out=3)),
+            ("cache", lambda: vkb.rope_append(None, table, ln, q, q, q)), ("cache", lambda: vkb.kv_read(None, table, i32, i32)),
+            ("seq", lambda: vkb.kv_read(cache, table, None, i32)), ("pos", lambda: vkb.kv_read(cache, table, i32, None)),
+            ("table", lambda: vkb.kv_read(cache, None, i32, i32)),
+            ("q", lambda: vkb.attention(cache, table, ln, None)), ("table", lambda: vkb.attention(cache, None, ln, q)),
+            ("lens", lambda: vkb.attention(cache, table, None, q)), ("cu", lambda: vkb.attention(cache, table, ln, q, cu=[0, 1, 2])),
+            ("out", lambda: vkb.attention(cache, table, ln, q, out=0)), ("work", lambda: vkb.attention(cache, table, ln, q, work=4096)),
+            ("window", lambda: vkb.attention(cache, table, ln, q, window=(1 << 32) + 5)), ("window", lambda: vkb.attention(cache, table, ln, q, window=-1)),
+            ("u", lambda: vkb.sample(x, None)), ("top_k", lambda: vkb.sample(x, u, top_k=40)), ("temperature", lambda: vkb.sample(x, u, 0.7)),
+            ("prob", lambda: vkb.sample(x, u, prob=1)), ("token", lambda: vkb.sample(x, u, token=1)), ("v", lambda: vkb.KvCache(cache.k, None, x, x)),
+            ("scales", lambda: vkb.KvCache(cache.k, cache.v, None, cache.v_scale))):
+        with pytest.raises(vkb.VkbError, match=rf"\b{name}\b"):
+            call()

@@ -38,6 +38,11 @@ def _handle(stream, dev: int) -> int:
     return _raw_stream(dev) if stream is None else stream.cuda_stream
 
 
+def _tensor(where: str, name: str, t) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise _Refused(where, f"{name} must be a tensor")
+
+
 def _device(where: str, x) -> int:
     """x's device index, which must be the current CUDA device."""
     dev = x.get_device()
@@ -77,9 +82,12 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
-def _array(where: str, name: str, t, n: int, dtype, dev: int) -> None:
-    """t (or None) is a contiguous [n] array on the device."""
-    if t is not None and (t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or t.get_device() != dev or not t.is_contiguous()):
+def _array(where: str, name: str, t, n: int, dtype, dev: int, optional: bool = False) -> None:
+    """t (or None, where it is optional) is a contiguous [n] array on the device."""
+    if t is None and optional:
+        return
+    _tensor(where, name, t)
+    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or t.get_device() != dev or not t.is_contiguous():
         raise _Refused(where, f"{name} must be contiguous {dtype} [{n}] on the tensors' device")
 
 
@@ -89,6 +97,7 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6, y=None, residual_out=N
     type or None, codes or None, scales or None): with q8 also y in the Q8 format (int8 [T][d], fp16 [T][d / 32]), which
     dequant() reads. residual_out may be residual."""
     w = "rms_norm"
+    _tensor(w, "x", x)
     dt = _DT.get(x.dtype)
     if x.dim() != 2 or dt is None or (x.shape[1] > 1 and x.stride(1) != 1):
         raise _Refused(w, "x must be [T][d] fp16, bf16 or fp32 with adjacent columns")
@@ -99,18 +108,19 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6, y=None, residual_out=N
     _array(w, "weight", weight, d, x.dtype, dev)
     res_dt = 0
     if residual is not None:
+        _tensor(w, "residual", residual)
         res_dt = _DT.get(residual.dtype)
         if res_dt is None or residual.shape != x.shape or residual.get_device() != dev or not residual.is_contiguous():
             raise _Refused(w, "residual must be contiguous [T][d] fp16, bf16 or fp32 on x's device")
         if residual_out is None:
             residual_out = _made(residual, stream)
-        elif residual_out.dtype != residual.dtype or residual_out.shape != x.shape or residual_out.get_device() != dev or not residual_out.is_contiguous():
+        elif not isinstance(residual_out, torch.Tensor) or residual_out.dtype != residual.dtype or residual_out.shape != x.shape or residual_out.get_device() != dev or not residual_out.is_contiguous():
             raise _Refused(w, "residual_out must be like residual")
     elif residual_out is not None:
         raise _Refused(w, "residual_out without residual")
     if y is None:
         y = _made(x, stream)
-    elif y.dtype != x.dtype or y.shape != x.shape or y.get_device() != dev or not y.is_contiguous():
+    elif not isinstance(y, torch.Tensor) or y.dtype != x.dtype or y.shape != x.shape or y.get_device() != dev or not y.is_contiguous():
         raise _Refused(w, "y must be contiguous [T][d] of x's type")
     q = s = None
     if q8:
@@ -168,12 +178,14 @@ class KvCache:
 
     def __init__(self, k, v, k_scale, v_scale):
         w = "KvCache"
+        _tensor(w, "k", k)
+        _tensor(w, "v", v)
         if k.dim() != 4 or k.dtype != torch.uint8 or not k.is_contiguous() or not k.is_cuda:
             raise _Refused(w, "k must be contiguous uint8 [pages][heads][page][dim] on a CUDA device")
         if v.dtype != torch.uint8 or v.shape != k.shape or v.device != k.device or not v.is_contiguous():
             raise _Refused(w, "v must be like k")
         for s in (k_scale, v_scale):
-            if s.dtype != torch.float32 or s.shape != k.shape[:2] or s.device != k.device or not s.is_contiguous():
+            if not isinstance(s, torch.Tensor) or s.dtype != torch.float32 or s.shape != k.shape[:2] or s.device != k.device or not s.is_contiguous():
                 raise _Refused(w, "scales must be contiguous fp32 [pages][heads] on k's device")
         pages, self.heads, self.page, self.dim = k.shape
         if self.page not in PAGES:
@@ -192,6 +204,11 @@ class KvCache:
         return cls(*codes, *[torch.zeros((pages, heads), dtype=torch.float32, device=device) for _ in range(2)])
 
 
+def _cache(where: str, cache) -> None:
+    if not isinstance(cache, KvCache):
+        raise _Refused(where, "cache must be a KvCache")
+
+
 def _rows(where: str, name: str, x, heads: int, dim: int, dev: int) -> int:
     """Row stride of x [T][heads][dim], whose heads are adjacent."""
     n, st = x.shape, x.stride()
@@ -202,6 +219,7 @@ def _rows(where: str, name: str, x, heads: int, dim: int, dev: int) -> int:
 
 def _batch(where: str, table, lens, cu, T: int, dev: int) -> int:
     """The number of sequences."""
+    _tensor(where, "table", table)
     if table.dim() != 2 or table.dtype != torch.int32 or not table.is_contiguous() or table.get_device() != dev or not table.numel():
         raise _Refused(where, "table must be contiguous int32 [B][pages] on the cache's device")
     B = table.shape[0]
@@ -221,7 +239,12 @@ def rope_append(cache: KvCache, table, lens, q, k, v, turns=None, cu=None, pos=N
     pos int32 [T] rotary positions (None: the place in the sequence), turns from rope_turns() (None: no rotation).
     q None: append only."""
     w = "rope_append"
+    _cache(w, cache)
+    _tensor(w, "k", k)
+    _tensor(w, "v", v)
     dev = _device(w, k)
+    if k.dim() != 3:
+        raise _Refused(w, "k must be [T][heads][dim]")
     T, heads, dim = k.shape[0], cache.heads, cache.dim
     dt, lay = _DT.get(k.dtype), _LAYOUT.get(layout)
     if dev != cache.device_index:
@@ -232,15 +255,17 @@ def rope_append(cache: KvCache, table, lens, q, k, v, turns=None, cu=None, pos=N
         raise _Refused(w, "k and v must be fp16, bf16 or fp32, alike")
     ldk, ldv = _rows(w, "k", k, heads, dim, dev), _rows(w, "v", v, heads, dim, dev)
     B = _batch(w, table, lens, cu, T, dev)
-    _array(w, "pos", pos, T, torch.int32, dev)
+    _array(w, "pos", pos, T, torch.int32, dev, optional=True)
     rot = 0
     if turns is not None:
-        rot = 2 * turns.shape[0]
+        _tensor(w, "turns", turns)
+        rot = 2 * turns.numel()
         if rot > dim or rot == 0:
             raise _Refused(w, "turns must be int64 [rot / 2] with 0 < rot <= dim")
         _array(w, "turns", turns, rot // 2, torch.int64, dev)
     hq = ldq = ldo = 0
     if q is not None:
+        _tensor(w, "q", q)
         if q.dim() != 3 or q.shape[0] != T or q.dtype != k.dtype:
             raise _Refused(w, "q must be [T][q_heads][dim] with k's rows and type")
         hq = q.shape[1]
@@ -249,7 +274,7 @@ def rope_append(cache: KvCache, table, lens, q, k, v, turns=None, cu=None, pos=N
             q_out = _made(q, stream)
             ldo = hq * dim
         else:
-            if q_out.dtype != q.dtype or q_out.shape != q.shape:
+            if not isinstance(q_out, torch.Tensor) or q_out.dtype != q.dtype or q_out.shape != q.shape:
                 raise _Refused(w, "q_out must be like q")
             ldo = _rows(w, "q_out", q_out, hq, dim, dev)
     elif q_out is not None:
@@ -264,6 +289,9 @@ def rope_append(cache: KvCache, table, lens, q, k, v, turns=None, cu=None, pos=N
 def kv_read(cache: KvCache, table, seq, pos, dtype=torch.float16, stream=None):
     """Cached tokens as values: (k, v) [n][heads][dim] of tokens pos[i] of sequences seq[i] (int32)."""
     w = "kv_read"
+    _cache(w, cache)
+    _tensor(w, "table", table)
+    _tensor(w, "seq", seq)
     dev = _device(w, seq)
     if dev != cache.device_index or seq.dim() != 1 or dtype not in _DT:
         raise _Refused(w, "seq and pos must be [n] on the cache's device, dtype fp16, bf16 or fp32")
@@ -293,6 +321,10 @@ def attention(cache: KvCache, table, lens, q, cu=None, scale: float | None = Non
     only the last `window` keys up to a row's own position. work: attention_workspace() (made here when not given, at
     the cost of an allocation and a memset)."""
     w = "attention"
+    _cache(w, cache)
+    _tensor(w, "q", q)
+    if not 0 <= window <= 0x7fffffff:
+        raise _Refused(w, "window must be 0 (none) or a number of keys below 2^31")
     dev = _device(w, q)
     if dev != cache.device_index or q.dim() != 3:
         raise _Refused(w, "q must be [T][q_heads][dim] on the cache's device")
@@ -307,13 +339,13 @@ def attention(cache: KvCache, table, lens, q, cu=None, scale: float | None = Non
         out = _made(q, stream)
         ldo = hq * cache.dim
     else:
-        if out.shape != q.shape or out.dtype != q.dtype:
+        if not isinstance(out, torch.Tensor) or out.shape != q.shape or out.dtype != q.dtype:
             raise _Refused(w, "out must be like q")
         ldo = _rows(w, "out", out, hq, cache.dim, dev)
     if work is None:
         with _on(stream):
             work = attention_workspace(cache)
-    elif work.get_device() != dev or not work.is_contiguous():
+    elif not isinstance(work, torch.Tensor) or work.get_device() != dev or not work.is_contiguous():
         raise _Refused(w, "work must be attention_workspace()'s tensor on the cache's device")
     check(lib().vkb_attention(cache._ref, table.data_ptr(), table.shape[1], lens.data_ptr(), _p(cu), B, T, _DT[q.dtype],
                               q.data_ptr(), ldq, out.data_ptr(), ldo, hq, cache.dim ** -0.5 if scale is None else scale,
@@ -327,16 +359,17 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, toke
     temperature, top_p, min_p fp32 [B], top_k int32 [B] (None: off). Returns (token int32 [B], its probability among the
     kept tokens fp32 [B]). The rules: include/vkb.h."""
     w = "sample"
+    _tensor(w, "logits", logits)
     dt = _DT.get(logits.dtype)
     if logits.dim() != 2 or dt is None or logits.shape[1] == 0 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise _Refused(w, "logits must be [B][V] fp16, bf16 or fp32 with adjacent columns")
     B, V = logits.shape
     dev, f32 = _device(w, logits), torch.float32
     _array(w, "u", u, B, f32, dev)
-    _array(w, "temperature", temperature, B, f32, dev)
-    _array(w, "top_k", top_k, B, torch.int32, dev)
-    _array(w, "top_p", top_p, B, f32, dev)
-    _array(w, "min_p", min_p, B, f32, dev)
+    _array(w, "temperature", temperature, B, f32, dev, optional=True)
+    _array(w, "top_k", top_k, B, torch.int32, dev, optional=True)
+    _array(w, "top_p", top_p, B, f32, dev, optional=True)
+    _array(w, "min_p", min_p, B, f32, dev, optional=True)
     if prob is None:
         prob = _made(u, stream)
     else:
