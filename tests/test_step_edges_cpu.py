@@ -1,6 +1,7 @@
 """Edge cases of the decode-step operators' boundary that need no GPU."""
 import math
 import os
+import re
 
 import pytest
 
@@ -47,3 +48,11 @@ def test_arguments_that_are_no_tensors_are_refused():
                        "cache": lambda: vkb.attention(None, x, x, x), "k": lambda: vkb.KvCache(None, x, x, x)}.items():
         with pytest.raises(vkb.VkbError, match=name):
             call()
+
+
+def test_grids_ask_the_device_for_its_sms():
+    root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "volta-kernel-bakeoff_b200", "csrc")
+    for name in ("norm.cu", "kv_cache.cu", "attention.cu", "sample.cu"):
+        with open(os.path.join(root, name)) as f:
+            code = [line.split("//")[0] for line in f]
+        assert not any(re.search(r"\b148\b", line) for line in code), name

@@ -265,3 +265,23 @@ def test_arguments_that_are_no_tensors_are_refused(cuda):
             ("scales", lambda: vkb.KvCache(cache.k, cache.v, None, cache.v_scale))):
         with pytest.raises(vkb.VkbError, match=rf"\b{name}\b"):
             call()
+
+
+# ---- reading the cache back -------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("x_dt", ["float16", "bfloat16", "float32"])
+def test_kv_read_of_more_tokens_than_the_grid_has_warps(cuda, x_dt):
+    """One rounding of code x scale (exact in fp32: 8 bits times 24, rounded once), whatever the number of tokens."""
+    import torch
+    lens = [70, 33]
+    cache, table, _ = make_cache(lens, 2, 48, 16)
+    g = gen(4)
+    n = 16 * 8 * torch.cuda.get_device_properties(0).multi_processor_count * 2 + 5
+    seq = torch.randint(0, 2, (n,), generator=g, device="cuda", dtype=torch.int32)
+    pos = (torch.rand(n, generator=g, device="cuda") * torch.tensor(lens, device="cuda")[seq.long()]).to(torch.int32)
+    got = vkb.kv_read(cache, table, seq, pos, dtype=dt(x_dt))
+    both = [values(cache, table, b, m) for b, m in enumerate(lens)]
+    for i in range(2):
+        want = torch.stack([torch.nn.functional.pad(both[b][i], (0, 0, 0, 0, 0, 70 - lens[b])) for b in range(2)])[seq.long(), pos.long()]
+        assert torch.equal(got[i], want.float().to(dt(x_dt)))
+    assert vkb.device_status() == 0

@@ -471,8 +471,10 @@ extern "C" int vkb_kv_read(const vkb_kv_cache_t* c, const int32_t* table, int ta
     if (!seq || !pos || !k || !v || !aligned_to(k, 16) || !aligned_to(v, 16)) return VKB_EINVAL;
     const ReadArgs a{{(const uint8_t*)c->k, (const uint8_t*)c->v}, {c->k_scale, c->v_scale}, {k, v}, table, seq, pos,
                      c->pages, c->heads, c->page, c->dim, table_ld, B, n};
-    const long long want = ((long long)n + 7) / 8;
-    const dim3 grid((unsigned)(want < 148 * 16 ? want : 148 * 16), 2);
+    int dev = 0;
+    if (int r = current_device(&dev)) return r;
+    const long long want = ((long long)n + 7) / 8, most = 16ll * device_info(dev).sm_count;
+    const dim3 grid((unsigned)(want < most ? want : most), 2);
     auto kern = dt == VKB_DT_F16 ? kv_read_kernel<VKB_DT_F16>
                 : dt == VKB_DT_BF16 ? kv_read_kernel<VKB_DT_BF16> : kv_read_kernel<VKB_DT_F32>;
     return launch_pdl(kern, grid, dim3(256), 0, (cudaStream_t)stream, 1, a);
