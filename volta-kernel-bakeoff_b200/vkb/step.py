@@ -86,8 +86,7 @@ def _array(where: str, name: str, t, n: int, dtype, dev: int, optional: bool = F
     """t (or None, where it is optional) is a contiguous [n] array on the device."""
     if t is None and optional:
         return
-    _tensor(where, name, t)
-    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or t.get_device() != dev or not t.is_contiguous():
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or t.get_device() != dev or not t.is_contiguous():
         raise _Refused(where, f"{name} must be contiguous {dtype} [{n}] on the tensors' device")
 
 
@@ -204,9 +203,7 @@ class KvCache:
         return cls(*codes, *[torch.zeros((pages, heads), dtype=torch.float32, device=device) for _ in range(2)])
 
 
-def _cache(where: str, cache) -> None:
-    if not isinstance(cache, KvCache):
-        raise _Refused(where, "cache must be a KvCache")
+_NO_CACHE = "cache must be a KvCache"
 
 
 def _rows(where: str, name: str, x, heads: int, dim: int, dev: int) -> int:
@@ -219,8 +216,7 @@ def _rows(where: str, name: str, x, heads: int, dim: int, dev: int) -> int:
 
 def _batch(where: str, table, lens, cu, T: int, dev: int) -> int:
     """The number of sequences."""
-    _tensor(where, "table", table)
-    if table.dim() != 2 or table.dtype != torch.int32 or not table.is_contiguous() or table.get_device() != dev or not table.numel():
+    if not isinstance(table, torch.Tensor) or table.dim() != 2 or table.dtype != torch.int32 or not table.is_contiguous() or table.get_device() != dev or not table.numel():
         raise _Refused(where, "table must be contiguous int32 [B][pages] on the cache's device")
     B = table.shape[0]
     _array(where, "lens", lens, B, torch.int32, dev)
@@ -239,12 +235,11 @@ def rope_append(cache: KvCache, table, lens, q, k, v, turns=None, cu=None, pos=N
     pos int32 [T] rotary positions (None: the place in the sequence), turns from rope_turns() (None: no rotation).
     q None: append only."""
     w = "rope_append"
-    _cache(w, cache)
-    _tensor(w, "k", k)
-    _tensor(w, "v", v)
+    if not isinstance(cache, KvCache):
+        raise _Refused(w, _NO_CACHE)
+    if not isinstance(k, torch.Tensor) or not isinstance(v, torch.Tensor) or k.dim() != 3:
+        raise _Refused(w, "k and v must be tensors [T][heads][dim]")
     dev = _device(w, k)
-    if k.dim() != 3:
-        raise _Refused(w, "k must be [T][heads][dim]")
     T, heads, dim = k.shape[0], cache.heads, cache.dim
     dt, lay = _DT.get(k.dtype), _LAYOUT.get(layout)
     if dev != cache.device_index:
@@ -258,15 +253,13 @@ def rope_append(cache: KvCache, table, lens, q, k, v, turns=None, cu=None, pos=N
     _array(w, "pos", pos, T, torch.int32, dev, optional=True)
     rot = 0
     if turns is not None:
-        _tensor(w, "turns", turns)
-        rot = 2 * turns.numel()
+        rot = 2 * turns.numel() if isinstance(turns, torch.Tensor) else 0
         if rot > dim or rot == 0:
             raise _Refused(w, "turns must be int64 [rot / 2] with 0 < rot <= dim")
         _array(w, "turns", turns, rot // 2, torch.int64, dev)
     hq = ldq = ldo = 0
     if q is not None:
-        _tensor(w, "q", q)
-        if q.dim() != 3 or q.shape[0] != T or q.dtype != k.dtype:
+        if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.shape[0] != T or q.dtype != k.dtype:
             raise _Refused(w, "q must be [T][q_heads][dim] with k's rows and type")
         hq = q.shape[1]
         ldq = _rows(w, "q", q, hq, dim, dev)
@@ -289,13 +282,14 @@ def rope_append(cache: KvCache, table, lens, q, k, v, turns=None, cu=None, pos=N
 def kv_read(cache: KvCache, table, seq, pos, dtype=torch.float16, stream=None):
     """Cached tokens as values: (k, v) [n][heads][dim] of tokens pos[i] of sequences seq[i] (int32)."""
     w = "kv_read"
-    _cache(w, cache)
-    _tensor(w, "table", table)
-    _tensor(w, "seq", seq)
+    if not isinstance(cache, KvCache):
+        raise _Refused(w, _NO_CACHE)
+    if not isinstance(seq, torch.Tensor):
+        raise _Refused(w, "seq must be a tensor")
     dev = _device(w, seq)
     if dev != cache.device_index or seq.dim() != 1 or dtype not in _DT:
         raise _Refused(w, "seq and pos must be [n] on the cache's device, dtype fp16, bf16 or fp32")
-    if table.dim() != 2 or table.dtype != torch.int32 or not table.is_contiguous() or table.get_device() != dev or not table.numel():
+    if not isinstance(table, torch.Tensor) or table.dim() != 2 or table.dtype != torch.int32 or not table.is_contiguous() or table.get_device() != dev or not table.numel():
         raise _Refused(w, "table must be contiguous int32 [B][pages] on the cache's device")
     n = seq.shape[0]
     _array(w, "seq", seq, n, torch.int32, dev)
@@ -321,8 +315,10 @@ def attention(cache: KvCache, table, lens, q, cu=None, scale: float | None = Non
     only the last `window` keys up to a row's own position. work: attention_workspace() (made here when not given, at
     the cost of an allocation and a memset)."""
     w = "attention"
-    _cache(w, cache)
-    _tensor(w, "q", q)
+    if not isinstance(cache, KvCache):
+        raise _Refused(w, _NO_CACHE)
+    if not isinstance(q, torch.Tensor):
+        raise _Refused(w, "q must be a tensor")
     if not 0 <= window <= 0x7fffffff:
         raise _Refused(w, "window must be 0 (none) or a number of keys below 2^31")
     dev = _device(w, q)
