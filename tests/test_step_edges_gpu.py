@@ -285,3 +285,25 @@ def test_kv_read_of_more_tokens_than_the_grid_has_warps(cuda, x_dt):
         want = torch.stack([torch.nn.functional.pad(both[b][i], (0, 0, 0, 0, 0, 70 - lens[b])) for b in range(2)])[seq.long(), pos.long()]
         assert torch.equal(got[i], want.float().to(dt(x_dt)))
     assert vkb.device_status() == 0
+
+
+# ---- sizes near 2^31 --------------------------------------------------------------------------------------------------
+
+def test_rms_norm_of_2_31_rows(cuda):
+    """The most rows that an int holds, one element each (x / sqrt(x x) is its sign); more are refused, not cut."""
+    import torch
+    T = (1 << 31) - 1
+    x = torch.full((T + 10, 1), 3.0, dtype=torch.float16, device="cuda")
+    x[T - 1] = -2.0
+    w = torch.full((1,), 0.5, dtype=torch.float16, device="cuda")
+    y, *_ = vkb.rms_norm(x[:T], w, eps=0.0)
+    assert float(y[-1]) == -0.5 and int((y[:-1] == 0.5).sum()) == T - 1
+    with pytest.raises(vkb.VkbError, match="2\\^31"):
+        vkb.rms_norm(x, w)
+
+
+def test_sample_refuses_what_an_int_does_not_hold(cuda):
+    import torch
+    wide = torch.zeros((1, (1 << 32) + 5), dtype=torch.float16, device="cuda")
+    with pytest.raises(vkb.VkbError, match="2\\^31"):
+        vkb.sample(wide, torch.zeros(1, device="cuda"))

@@ -184,12 +184,12 @@ template <int X, int R> static int norm_launch(const NormArgs& a, bool vec, cuda
     // once (B200, bf16 in, residual and out: 8191 rows of 2560 take 34 us, 37 with a block per row; 2047 and 2048 rows 11 us
     // either way).
     if (vec && n > 64 && n <= 32 * NORM_WNV && a.T >= 2048) {
-        const dim3 grid((unsigned)((a.T + 3) / 4)), block(32, 4);
+        const dim3 grid((unsigned)((a.T - 1) / 4 + 1)), block(32, 4);
         return launch_pdl(norm_vec_kernel<X, R, NORM_WNV, true>, grid, block, 0, st, 1, a);
     }
     const int tpr = n <= 64 ? 32 : min(1024, (n + 31) / 32 * 32);
     const int rows = tpr == 32 ? 4 : 1;
-    const dim3 grid((unsigned)((a.T + rows - 1) / rows)), block((unsigned)tpr, (unsigned)rows);
+    const dim3 grid((unsigned)((a.T - 1) / rows + 1)), block((unsigned)tpr, (unsigned)rows);
     return launch_pdl(vec ? norm_vec_kernel<X, R, NORM_NV, false> : norm_any_kernel<X, R>, grid, block, 0, st, 1, a);
 }
 

@@ -19,6 +19,7 @@ DT_F16, DT_BF16, DT_F32 = 0, 1, 2
 _DT = {torch.float16: DT_F16, torch.bfloat16: DT_BF16, torch.float32: DT_F32}
 _LAYOUT = {"half": 0, "interleaved": 1}
 PAGES = (16, 32, 64, 128)
+_INT = 0x7fffffff     # what the library's sizes hold
 
 
 class _Refused(VkbError):
@@ -102,8 +103,8 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6, y=None, residual_out=N
         raise _Refused(w, "x must be [T][d] fp16, bf16 or fp32 with adjacent columns")
     T, d = x.shape
     dev = _device(w, x)
-    if d == 0:
-        raise _Refused(w, "d must be positive")
+    if d == 0 or T > _INT or d > _INT:
+        raise _Refused(w, "d must be positive, T and d below 2^31")
     _array(w, "weight", weight, d, x.dtype, dev)
     res_dt = 0
     if residual is not None:
@@ -319,7 +320,7 @@ def attention(cache: KvCache, table, lens, q, cu=None, scale: float | None = Non
         raise _Refused(w, _NO_CACHE)
     if not isinstance(q, torch.Tensor):
         raise _Refused(w, "q must be a tensor")
-    if not 0 <= window <= 0x7fffffff:
+    if not 0 <= window <= _INT:
         raise _Refused(w, "window must be 0 (none) or a number of keys below 2^31")
     dev = _device(w, q)
     if dev != cache.device_index or q.dim() != 3:
@@ -360,6 +361,8 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, toke
     if logits.dim() != 2 or dt is None or logits.shape[1] == 0 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise _Refused(w, "logits must be [B][V] fp16, bf16 or fp32 with adjacent columns")
     B, V = logits.shape
+    if B > _INT or V > _INT:
+        raise _Refused(w, "B and V must be below 2^31")
     dev, f32 = _device(w, logits), torch.float32
     _array(w, "u", u, B, f32, dev)
     _array(w, "temperature", temperature, B, f32, dev, optional=True)
