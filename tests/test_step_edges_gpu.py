@@ -307,3 +307,51 @@ def test_sample_refuses_what_an_int_does_not_hold(cuda):
     wide = torch.zeros((1, (1 << 32) + 5), dtype=torch.float16, device="cuda")
     with pytest.raises(vkb.VkbError, match="2\\^31"):
         vkb.sample(wide, torch.zeros(1, device="cuda"))
+
+
+# ---- variants that larger calls take ----------------------------------------------------------------------------------
+
+MANY = [(2048, 520), (2049, 2560), (2050, 544), (2051, 1032)]     # a row per warp: filled lanes and not, last blocks of 1 to 4 rows
+
+
+@pytest.mark.parametrize("T,d", MANY)
+@pytest.mark.parametrize("x_dt,res_dt", [("float16", "float32"), ("bfloat16", "bfloat16"), ("float32", "float16"), ("float32", None), ("bfloat16", None)])
+def test_rms_norm_of_many_rows(cuda, T, d, x_dt, res_dt):
+    """A lane's share of the sum is up to 80 squares one after another, 5 additions over the lanes: 85 u32, halved by the root,
+    and five roundings: within the bound of (d / 1024 + 60) u32 that the rows per block are held to."""
+    from test_step_gpu import test_rms_norm
+    test_rms_norm(cuda, T, d, x_dt, res_dt)
+
+
+@pytest.mark.parametrize("T,d", [(1, 32), (33, 2560), (3, 2080), (4, 16416)] + MANY[1:3])
+@pytest.mark.parametrize("x_dt,res_dt", [("float16", "float32"), ("bfloat16", "bfloat16"), ("float32", "float16"), ("float16", None)])
+def test_rms_norm_q8_with_residual(cuda, T, d, x_dt, res_dt):
+    """Codes and scales of the exact y as in test_rms_norm_q8, for every kernel, and y and the residual as without them."""
+    import torch
+    g = gen(T + d)
+    x = torch.randn((T, d), generator=g, device="cuda").to(dt(x_dt))
+    w = (1 + 0.3 * torch.randn(d, generator=g, device="cuda")).to(dt(x_dt))
+    res = None if res_dt is None else (4 * torch.randn((T, d), generator=g, device="cuda")).to(dt(res_dt))
+    y, r, q, s = vkb.rms_norm(x, w, res, q8=True)
+    y2, r2, *_ = vkb.rms_norm(x, w, res)
+    assert torch.equal(y, y2) and (res is None or torch.equal(r, r2))
+    R = x.double() + (res.double() if res is not None else 0)
+    B = (R / torch.sqrt(R.square().mean(1, keepdim=True) + 1e-6) * w.double()).view(T, -1, 32)
+    amax = B.abs().amax(-1)
+    assert bool(((s.double() - amax / 127).abs() <= amax / 127 * (2.0 ** -11 + 1e-5) + 2.0 ** -24).all())
+    val, step = vkb.dequant(vkb.FMT_Q8, q, s, T, d).double().view(T, -1, 32), s.double()[..., None]
+    assert bool(((val - B).abs() <= step * (0.5 + 127 * 2.0 ** -11 + 1e-3) + 2.0 ** -11 * B.abs() + 2.0 ** -24).all())
+
+
+@pytest.mark.parametrize("lens,news,heads,hq,dim,rot,page,layout,x_dt", [
+    ([200, 64], [200, 64], 2, 4, 256, 256, 64, "half", "float16"),             # 39 tokens at a time
+    ([300], [230], 1, 2, 256, 64, 128, "interleaved", "bfloat16"),
+    ([130, 100], [125, 60], 2, 2, 192, 192, 64, "half", "bfloat16"),           # 52
+    ([260, 128], [250, 128], 1, 1, 128, 128, 128, "half", "float16"),          # 77
+    ([128], [128], 1, 1, 80, 40, 128, "interleaved", "float32"),               # 121
+])
+def test_rope_append_of_pages_that_take_several_turns(cuda, lens, news, heads, hq, dim, rot, page, layout, x_dt):
+    """Pages whose new tokens do not fit a block's shared memory at once."""
+    from test_step_gpu import test_rope_append
+    assert max(min(n, page) for n in news) > 40960 // (4 * (dim + 4))
+    test_rope_append(cuda, lens, news, heads, hq, dim, rot, page, layout, x_dt)
