@@ -71,10 +71,15 @@ template <typename T>
 static int attn_dispatch(const vkb_kv_cache_t* c, const AttnArgs& a, int dev, cudaStream_t st) {
     // Query rows per sequence and kv head, on average: the token kernel with the smallest tile that holds them. More rows
     // than its largest tile go to the prompt kernel, whose tile reads the keys once for 256 rows (128 at dimension 256), unless
-    // the call is so small that the token kernel's many small items keep the SMs busier. Measured (32 q heads on 8,
-    // dimension 128, B200): one sequence of 8192 keys, 64 rows 40 us against 48, 256 rows 81 against 108, 512 rows 130
-    // against 98; 16 sequences of 1500 keys, 64 rows 83 against 66; 16 q heads on 2, dimension 256: one of 8192 keys, 256 rows 48
-    // against 214, 16 of 1500 keys, 128 rows 72 against 101, 384 rows 174 against 107.
+    // the call is so small that the token kernel's many small items keep the SMs busier. Measured (token kernel against prompt
+    // kernel, us, B200): 32 q heads on 8, dimension 128: one sequence of 8192 keys, 64 rows 39 against 50, 256 rows 79 against
+    // 115, 512 rows 131 against 99; 16 sequences of 1500 keys, 36 rows 76 against 65, 64 rows 81 against 67. Dimension 64: one of
+    // 8192 keys, 256 rows 65 against 66, 512 rows 108 against 64; 16 of 1500, 36 rows 62 against 54; 32 q heads on 2, 16 of 1500,
+    // 64 rows 31 against 32, 128 rows 42 against 36. 16 q heads on 2, dimension 256: one of 8192 keys, 256 rows 48 against 214,
+    // 16 of 1500 keys, 128 rows 72 against 101, 384 rows 174 against 107.
+    // All of these are sequences alike. The lengths are on the device, so one kernel serves a call whose sequences differ, and
+    // the mean says little there: 63 single tokens behind 4000 keys with a chunk of 2048 take 558 us (token kernel 1035), apart
+    // 104 and 204; 255 behind 1000 with a prompt of 1024 556 us (prompt kernel 608), apart 151 and 76.
     const long long rows = ((long long)a.T + a.B - 1) / a.B * a.G;
     const bool few = (long long)a.T * a.G * a.heads <= (c->dim > 128 ? 4096 : 2560);
     switch (attn_dt(c->dim)) {

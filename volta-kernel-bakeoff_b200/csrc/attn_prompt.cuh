@@ -23,7 +23,9 @@
 //   warps 12-15   convert codes: global loads of 16 codes (past L1: each is read once), two tiles ahead in registers, to
 //                 128-byte swizzled fp16 tiles (K: K-major B operand; V: the same bytes are the MN-major B operand of P V)
 // Measured on a B200 (32 q heads on 8, dimension 128): 4096 tokens behind 12288 take 1.21 ms, 795 TFLOP/s on the causal
-// pairs; the tensor pipe is busy for 35 % of it, the exponentials for a third: bound by the softmax warps' issue.
+// pairs; the tensor pipe is busy for 36 % of it, the exponentials for a third, and a
+// scheduler issues 0.41 instructions per cycle: bound by latency, two softmax warps per scheduler with one dependent chain per
+// tile each (load of S, multiply-add, exponential, pack, store of P).
 #pragma once
 
 #include "attn_token.cuh"

@@ -17,7 +17,7 @@
 // reaches the second product through movmatrix. tcgen05 has nothing to add: with 8 rows its tiles would be empty.
 // p' is rounded once, to fp16, for the product. It is computed against the M of the keys before; only where one passes
 // 2^(8 + 4) the warp finds the new maximum, rescales and computes it again. vs below 2^-30 V counts as that.
-// Measured on a B200 (32 q heads on 8, dimension 128): 64 sequences of 1 to 8192 tokens 110 us, 4.6 TB/s of codes; one
+// Measured on a B200 (32 q heads on 8, dimension 128): 64 sequences of 1 to 8192 tokens 112 us, 4.5 TB/s of codes; one
 // sequence of 131073, 24 heads on 4, 40 us, 3.4 TB/s; one of 777 tokens 9.5 us from the first block's start to the last's end.
 // q: fp16 as it is; bf16 rows are scaled by a power of two into fp16's range first (exact but for values 2^-28 below the
 // row's largest).

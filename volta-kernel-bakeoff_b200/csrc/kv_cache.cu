@@ -11,10 +11,14 @@
 // (page, head, tensor) belongs to one block of threads, so nothing is atomic and the result does not depend on order.
 // Infinities are held as +-127 and do not enter the scale; NaN is held as 0.
 //
-// HBM-bound for prompts (every element read once, q written once, codes written once; a token's cosines are made once per
-// block and the turned k of a page stays in shared memory between the search for its maximum and its codes),
-// latency-bound for single tokens: one launch for q, k and v, blocks of 128 threads. Measured on a B200: 10492 tokens of
-// ragged prompts, 16 q heads on 4 of 256, pages of 16, in 93 us (2.5 TB/s), read back in 23 us.
+// For prompts q is read and written once, and k and v are read once where a page's values fit 40 KB of shared memory as fp32
+// (page x (dim + 4) up to 10240): a token's cosines are made once per block, and the turned k stays there between the search for
+// its maximum and its codes. Larger pages go in turns and read k and v twice. Single tokens: latency; one launch for q, k and
+// v, blocks of 128 threads.
+// Measured on a B200: 10492 tokens of ragged prompts, 16 q heads on 4 of 256 (36 us of bytes): pages of 16 in 92 us, bound by
+// the start of each block (its sequence, page and scale, one load after another), pages of 32 in 122 (20 KB per block: fewer
+// at a time), 64 and 128 in 159 (two and four turns). Read back in 21.5 us (10 us of bytes): a warp waits for a token's
+// sequence, position, page and scale one after another.
 #include <mutex>
 
 #include "step.cuh"
@@ -280,8 +284,9 @@ template <int DT> __global__ void __launch_bounds__(AP_THREADS) rope_append_kern
     const long long ph = (long long)id * a.heads + h;
     uint8_t* codes = a.codes[which] + ph * a.page * a.dim;
     const float before = held > 0 ? a.scale[which][ph] : 0.f;
-    // The tokens in turns of as many as shared memory holds, as fp32 (turned, for k): one turn but for the largest pages
-    // in fp32 rows of 128 x 256; where there is more than one, the second pass makes its values again.
+    // The tokens in turns of as many as shared memory holds, as fp32 (turned, for k): one turn where page x (dim + 4) x 4 bytes
+    // are at most 40 KB (of 256-wide heads 39 tokens, of 128-wide ones 77); where there is more than one, the second pass
+    // makes its values again.
     const int count = hi - lo, dv4 = a.dim + 4;   // 4 floats apart from a multiple of the banks
     float2* cs = reinterpret_cast<float2*>(ap_smem);
     float* vals = reinterpret_cast<float*>(ap_smem + 8 * a.cs_max);

@@ -776,7 +776,7 @@ template <int DT, int CL> static int launch_sample(const SampleArgs& a, int B, i
 }
 
 template <int DT> static int sample_cl(SampleArgs a, int B, int dev, cudaStream_t st) {
-    // blocks per row: slices of a few thousand logits where the batch is small enough for the SMs, larger ones otherwise
+    // Blocks per row, by the row's length alone: up to 4096 logits each until there are eight, whatever the batch.
     int cl = 1;
     while (cl < 8 && a.V > 4096 * cl) cl *= 2;
     a.slice = ((a.V + cl - 1) / cl + 7) / 8 * 8;
