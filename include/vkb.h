@@ -191,8 +191,9 @@ int vkb_kv_read(const vkb_kv_cache_t* cache, const int32_t* table, int table_ld,
 /* out[t][h] = sum_j softmax_j(scale * q[t][h] . k_j) v_j over the cache, query head h on kv head h / (q_heads / heads).
  * Query row i of a sequence's n rows is at position len - n + i and sees the keys at positions up to its own, with
  * window > 0 only the last `window` of them; a row that sees no key is zero. Table entries of pages that no row sees are
- * not looked at: pages that the window has passed may be given back. q and out: fp16 or bf16, 16-byte aligned rows. work: vkb_attention_work_bytes(dim) bytes (for the current device), 16-byte aligned, zeroed by the caller once
- * before its first use; calls leave it ready for the next one. Calls that overlap in time need a workspace each. */
+ * not looked at: pages that the window has passed may be given back. q and out: fp16 or bf16, 16-byte aligned rows. work:
+ * vkb_attention_work_bytes(dim) bytes (for the current device), 16-byte aligned, zeroed by the caller once before its
+ * first use; calls leave it ready for the next one. Calls that overlap in time need a workspace each. */
 size_t vkb_attention_work_bytes(int dim);
 int vkb_attention(const vkb_kv_cache_t* cache, const int32_t* table, int table_ld, const int32_t* lens,
                   const int32_t* cu, int B, int T, int dt, const void* q, long long ldq, void* out, long long ldo,
